@@ -249,9 +249,14 @@ def prepare(case, seed):
         r = random.Random(case["mix"] + 2)
         paths = [_path(r, case["nodes"], case["path"]) for _ in starts]
         s.path = _int([p + [-1] * (case["path"] - len(p)) for p in paths])
+        if own:  # the handles of the layers' pools, which an engine keeps
+            vr = _vr()
+            s.layers = vr.pool_array([_pool_of(vr, case, {n: x[i] for n, x in s.pool.items()}) for i in range(case["layers"])])
         return s
     s.pool = _empty_pool(case, blocks)
     s.q = _queries(case, seed)
+    if own:
+        s.handle = _pool_of(_vr(), case, s.pool)
     for b, n in enumerate(starts):
         _write(case, s.pool, s.tables[b], *_cached(case, seed, b, n + case["nodes"]))
     trees = _trees(case)
@@ -404,10 +409,9 @@ def _own(s):
     vr, c = _vr(), s.case
     if c["kind"] == "tree":
         numerics = vr.NUMERICS_3BIT if c["numerics"] == "3bit" else vr.NUMERICS_PLAIN
-        return vr.paged_tree_attention(_pool_of(vr, c, s.pool), s.tables, s.start, s.q, tree_mask=s.mask, tree_lens=s.lens, max_start_pos=s.max_start, numerics=numerics)
+        return vr.paged_tree_attention(s.handle, s.tables, s.start, s.q, tree_mask=s.mask, tree_lens=s.lens, max_start_pos=s.max_start, numerics=numerics)
     if c["kind"] == "accept":
-        layers = [_pool_of(vr, c, {n: x[i] for n, x in s.pool.items()}) for i in range(c["layers"])]
-        return vr.kv_accept(layers, s.tables, s.start, s.path, c["nodes"])
+        return vr.kv_accept(s.layers, s.tables, s.start, s.path, c["nodes"]).long()
     layout = vr.ROPE_HALF if c["layout"] == "half" else vr.ROPE_INTERLEAVED
     scaling = {"none": vr.ROPE_SCALE_NONE, "linear": vr.ROPE_SCALE_LINEAR, "base": vr.ROPE_SCALE_BASE, "bands": vr.ROPE_SCALE_BANDS, "yarn": vr.ROPE_SCALE_YARN}[c["scaling"]]
     q, k = vr.rope(s.pos, s.q, s.k, rope_dim=c["rope_dim"], base=c["base"], layout=layout, scaling=scaling, factor=c["factor"], trained_len=LENGTH,

@@ -186,6 +186,123 @@ int vspec_rocm_paged_decode_step(const VspecPagedAttnDesc* desc, const void* k_n
 int vspec_rocm_paged_decode_step_noalloc(const VspecPagedAttnDesc* desc, const void* k_new, const void* v_new,
                                          int32_t src_dtype);
 
+/* ---- a speculative step: a tree of drafted tokens, verified in one pass ----
+ * No counterpart in the reference.  A step drafts up to 64 nodes for every sequence, rotates
+ * their queries and keys by depth (vspec_rocm_rope), writes the keys and values behind the
+ * cached prefix (vspec_rocm_kv_append with start_pos and n_new = num_nodes, or
+ * vspec_rocm_kv_append_tokens), attends every node to the prefix and to the nodes that its mask
+ * names (vspec_rocm_paged_tree_attention), and moves the accepted path together
+ * (vspec_rocm_kv_accept).  Node j of sequence b lies in slot start_pos[b] + j. */
+
+/* Attention of the nodes.  Numerics per query row and key as
+ * vspec_rocm_paged_decode_attention; any GQA group. */
+typedef struct VspecTreeAttnDesc {
+    VspecPagedKV kv;                 /* head_dim 64 or 128, block_tokens a multiple of 16 */
+    uint32_t batch;
+    uint32_t num_q_heads;            /* multiple of kv.num_kv_heads */
+    uint32_t num_nodes;              /* N, rows a sequence of q, out and tree_mask: 1..64 */
+    const int32_t* block_tables;     /* device [batch][max_blocks_per_seq] */
+    uint32_t max_blocks_per_seq;
+    const int32_t* start_pos;        /* device [batch]: tokens before the tree, all visible to
+                                        every node; a negative one counts as 0 */
+    uint32_t max_start_pos;          /* host upper bound of start_pos: it plans the split (a
+                                        longer prefix is still read whole); 0: the table's
+                                        capacity */
+    const int32_t* tree_lens;        /* device [batch], nodes of each sequence (0..N; clamped),
+                                        or NULL: N each.  Rows past it come out as zeros */
+    const uint64_t* tree_mask;       /* device [batch][N]: bit j of row i lets node i see node j
+                                        (j < tree_lens[b]; its own bit included); NULL: a chain,
+                                        node i sees nodes 0..i.  A row that sees no token at
+                                        all comes out as zeros.  A node's keys and values reach
+                                        only the rows that see it, whatever their bits */
+    const void* q;                   /* device [batch][N][Hq][D] in io_dtype, 16-byte aligned */
+    void* out;                       /* device, as q */
+    int32_t io_dtype;                /* VSPEC_KV_F32 or VSPEC_KV_F16.  f16 rows are multiplied
+                                        with softmax weights rounded to f16 (and int4 values
+                                        rounded to f16); f32 rows keep about 22 bits */
+    float scale;                     /* <= 0: 1/sqrtf(D) */
+    int32_t numerics;                /* VSPEC_NUMERICS_PLAIN or VSPEC_NUMERICS_3BIT */
+    float clamp_alpha;               /* <= 0: 4.5 */
+    void* workspace;                 /* device scratch (no init needed) or NULL: library's */
+    size_t workspace_bytes;
+    void* stream;                    /* hipStream_t or NULL */
+    const int32_t* block_used;       /* as VspecPagedAttnDesc.block_used, or NULL; start_pos is
+                                        then the slot-space position of the first node, and the
+                                        blocks that hold nodes count them */
+} VspecTreeAttnDesc;
+
+size_t vspec_rocm_paged_tree_attention_workspace_bytes(const VspecTreeAttnDesc* desc);
+int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc);
+
+/* Keep the accepted path.  path: device int32 [batch][max_path], the accepted nodes of each
+ * sequence in order; the first entry outside 0..num_nodes-1 ends it.  Slot start_pos[b] + i
+ * gets what slot start_pos[b] + path[b][i] held before the call, K and V with scales and clamp
+ * flags, for every i before the end, in each of the num_kvs pools (one a layer: host array;
+ * the pools share dtype, geometry and block tables).  Any order of nodes is right, the same
+ * node twice included.  new_lens (device int32 [batch], or NULL) gets start_pos[b] plus the
+ * accepted nodes.  A slot outside the table or behind an invalid entry is neither read nor
+ * written.  The blocks written belong to their sequence alone.  max_path and num_nodes are at
+ * most 64. */
+int vspec_rocm_kv_accept(const VspecPagedKV* kvs, uint32_t num_kvs, uint32_t batch,
+                         const int32_t* block_tables, uint32_t max_blocks_per_seq,
+                         const int32_t* start_pos, const int32_t* path, uint32_t max_path,
+                         uint32_t num_nodes, int32_t* new_lens, void* stream);
+
+/* Rotary positions, given for each token (nodes at one depth share a position, not a slot).
+ * Pair i < rope_dim/2 of a row, elements (i, i + rope_dim/2) or (2i, 2i + 1), becomes
+ *   m (x1 cos a - x2 sin a), m (x1 sin a + x2 cos a),    a = position * f_i,
+ * the other elements of a row are copied.  Angles are reduced in 64 bits, products and sums are
+ * f32, each result is rounded once.  f_i = base^(-2i/rope_dim), for a longer context than the
+ * trained one stretched by
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(rope_dim / (rope_dim - 2)) in the place of base
+ *   BANDS   with t_i = trained_len f_i / 2 pi turns over the trained length: t_i <= low: f_i / factor;
+ *           t_i >= high: f_i; between them a mean of both, linear in t_i
+ *   YARN    pairs between those that turn `high` and `low` times over the trained length
+ *           (floor and ceiling of their index): a mean of f_i and f_i / factor, linear in i;
+ *           faster ones f_i, slower ones f_i / factor; m = 0.1 ln(factor) + 1
+ * m is 1 but for YARN, or `magnitude` where that is above 0.  inverse turns by -a with the
+ * same m: the gradient of the rotation. */
+enum { VSPEC_ROPE_HALF = 0, VSPEC_ROPE_INTERLEAVED = 1 };
+enum {
+    VSPEC_ROPE_SCALE_NONE = 0,
+    VSPEC_ROPE_SCALE_LINEAR = 1,
+    VSPEC_ROPE_SCALE_BASE = 2,
+    VSPEC_ROPE_SCALE_BANDS = 3,
+    VSPEC_ROPE_SCALE_YARN = 4
+};
+
+/* Rows of one operand, [num_tokens][num_heads][head_dim] with strides in elements (0: dense);
+ * the elements of a row are adjacent.  out is `in` with the same strides (in place), or memory
+ * that overlaps neither operand's rows. */
+typedef struct VspecRopeRows {
+    const void* in;                  /* device; NULL: no such operand */
+    void* out;
+    uint32_t num_heads;
+    int64_t in_token_stride, in_head_stride;
+    int64_t out_token_stride, out_head_stride;
+} VspecRopeRows;
+
+typedef struct VspecRopeDesc {
+    uint32_t num_tokens;
+    uint32_t head_dim;               /* 2..256 */
+    uint32_t rope_dim;               /* even, 2..head_dim */
+    int32_t dtype;                   /* VSPEC_KV_F32 or VSPEC_KV_F16 */
+    int32_t layout;                  /* VSPEC_ROPE_HALF or VSPEC_ROPE_INTERLEAVED */
+    int32_t inverse;
+    int32_t scaling;                 /* VSPEC_ROPE_SCALE_* */
+    uint32_t trained_len;            /* BANDS, YARN */
+    double base;                     /* above 1 */
+    double factor;                   /* at least 1 (NONE: unused) */
+    double low, high;                /* BANDS, YARN: turns, 0 < low < high */
+    double magnitude;                /* <= 0: the scaling's own */
+    const int32_t* positions;        /* device [num_tokens] */
+    VspecRopeRows q, k;
+    void* stream;                    /* hipStream_t or NULL */
+} VspecRopeDesc;
+
+int vspec_rocm_rope(const VspecRopeDesc* desc);
+
 /* Free the library workspaces that later, larger decodes replaced on the current device.
  * They are kept until this call because a captured HIP graph may still use them; call it
  * only when no such graph will be replayed again. */

@@ -52,6 +52,7 @@ extern "C" void vspec_rocm_set_error_(const char* msg) { set_err("%s", msg ? msg
 
 #include "kv_common.h"
 #include "append_row.h"
+#include "host.h"
 
 namespace {
 using namespace vkv;
@@ -1041,6 +1042,20 @@ int plan_decode(const VspecPagedAttnDesc* d, DecodePlan* pl, uint32_t most_heads
 }
 
 }  // namespace
+
+namespace vkv {
+
+void host_error(const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+}
+int host_check_kv(const VspecPagedKV* kv, const char* who, bool decode) { return check_kv(kv, who, decode); }
+void* host_workspace(size_t bytes) { return library_workspace(bytes); }
+int host_num_cus() { return num_cus(); }
+
+}  // namespace vkv
 
 // ---------------------------------------------------------------------------
 // C-ABI

@@ -18,6 +18,8 @@ LIB_PATH = Path(os.environ.get("VSPEC_ROCM_LIB", PKG_ROOT / "lib" / "libvspec_ro
 KV_F32, KV_F16, KV_INT4 = 0, 1, 2
 NUMERICS_PLAIN, NUMERICS_3BIT = 0, 1
 GATHER_RAW, GATHER_F32 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BASE, ROPE_SCALE_BANDS, ROPE_SCALE_YARN = 0, 1, 2, 3, 4
 KCTX_FLAG_PAGED = 1
 
 _vp = C.c_void_p
@@ -59,6 +61,65 @@ class VspecPagedAttnDesc(C.Structure):
         ("stream", _vp),
         ("block_used", _vp),
         ("min_ctx_len", C.c_uint32),
+    ]
+
+
+class VspecTreeAttnDesc(C.Structure):
+    _fields_ = [
+        ("kv", VspecPagedKV),
+        ("batch", C.c_uint32),
+        ("num_q_heads", C.c_uint32),
+        ("num_nodes", C.c_uint32),
+        ("block_tables", _vp),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("start_pos", _vp),
+        ("max_start_pos", C.c_uint32),
+        ("tree_lens", _vp),
+        ("tree_mask", _vp),
+        ("q", _vp),
+        ("out", _vp),
+        ("io_dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("numerics", C.c_int32),
+        ("clamp_alpha", C.c_float),
+        ("workspace", _vp),
+        ("workspace_bytes", C.c_size_t),
+        ("stream", _vp),
+        ("block_used", _vp),
+    ]
+
+
+class VspecRopeRows(C.Structure):
+    _fields_ = [
+        ("in_", _vp),
+        ("out", _vp),
+        ("num_heads", C.c_uint32),
+        ("in_token_stride", C.c_int64),
+        ("in_head_stride", C.c_int64),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+    ]
+
+
+class VspecRopeDesc(C.Structure):
+    _fields_ = [
+        ("num_tokens", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("rope_dim", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("layout", C.c_int32),
+        ("inverse", C.c_int32),
+        ("scaling", C.c_int32),
+        ("trained_len", C.c_uint32),
+        ("base", C.c_double),
+        ("factor", C.c_double),
+        ("low", C.c_double),
+        ("high", C.c_double),
+        ("magnitude", C.c_double),
+        ("positions", _vp),
+        ("q", VspecRopeRows),
+        ("k", VspecRopeRows),
+        ("stream", _vp),
     ]
 
 
@@ -159,6 +220,11 @@ SIGNATURES = {
     "vspec_rocm_paged_decode_attention": (C.c_int, [C.POINTER(VspecPagedAttnDesc)]),
     "vspec_rocm_paged_decode_step": (C.c_int, [C.POINTER(VspecPagedAttnDesc), _vp, _vp, C.c_int32]),
     "vspec_rocm_paged_decode_step_noalloc": (C.c_int, [C.POINTER(VspecPagedAttnDesc), _vp, _vp, C.c_int32]),
+    "vspec_rocm_paged_tree_attention_workspace_bytes": (C.c_size_t, [C.POINTER(VspecTreeAttnDesc)]),
+    "vspec_rocm_paged_tree_attention": (C.c_int, [C.POINTER(VspecTreeAttnDesc)]),
+    "vspec_rocm_kv_accept": (C.c_int, [C.POINTER(VspecPagedKV), C.c_uint32, C.c_uint32, _vp, C.c_uint32, _vp, _vp, C.c_uint32,
+                                       C.c_uint32, _vp, _vp]),
+    "vspec_rocm_rope": (C.c_int, [C.POINTER(VspecRopeDesc)]),
     "vspec_rocm_sync": (C.c_int, [_vp]),
     "vspec_rocm_last_error": (C.c_char_p, []),
     "vspec_rocm_device_count": (C.c_int, []),
@@ -309,6 +375,31 @@ class PagedPool:
                        if flags else None)
         else:
             self.ks = self.vs = self.kf = None
+
+    @classmethod
+    def over(cls, dtype: int, block_tokens: int, num_kv_heads: int, head_dim: int, k, v, ks=None, vs=None, kf=None):
+        """A pool over tensors that the caller holds, contiguous and in the layout above (their
+        element types may be any of the right total size; ks and vs for int4, kf optional)."""
+        self = cls.__new__(cls)
+        self.dtype, self.block_tokens, self.num_kv_heads, self.head_dim = dtype, block_tokens, num_kv_heads, head_dim
+        if dtype not in (KV_F32, KV_F16, KV_INT4):
+            raise ValueError("dtype")
+        row = {KV_F32: 4 * head_dim, KV_F16: 2 * head_dim, KV_INT4: head_dim // 2}[dtype]
+        block = num_kv_heads * block_tokens * row
+        self.num_blocks = k.numel() * k.element_size() // block
+        rows = self.num_blocks * num_kv_heads * block_tokens
+        want = [("k", k, rows * row), ("v", v, rows * row)]
+        if dtype == KV_INT4:
+            want += [("ks", ks, rows * (head_dim // 32) * 2), ("vs", vs, rows * (head_dim // 32) * 2)]
+            if kf is not None:
+                want.append(("kf", kf, rows // 16 * 4))
+        else:
+            ks = vs = kf = None
+        for name, t, size in want:
+            if t is None or not t.is_contiguous() or t.numel() * t.element_size() != size or t.device != k.device:
+                raise VspecRocmError(f"pool tensor {name}: need {size} contiguous bytes on {k.device}")
+        self.k, self.v, self.ks, self.vs, self.kf = k, v, ks, vs, kf
+        return self
 
     @property
     def device(self):
@@ -514,6 +605,155 @@ def paged_decode_step(pool: PagedPool, block_tables, ctx_lens, q, k_new, v_new, 
            "paged_decode_step")
     _hold(stream, bt, cl, bu, out)
     return out
+
+
+def _on_device(what, device, **tensors):
+    """Every tensor is on the device that the call runs on, which is the current one: the
+    launch goes to one of its streams."""
+    import torch
+
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise VspecRocmError(f"{what}: the data is on {device}, which is not the current GPU")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise VspecRocmError(f"{what}: {name} is on {t.device}, not on {device}")
+
+
+def _io_type(what, t):
+    import torch
+
+    if t.dtype == torch.float32:
+        return KV_F32
+    if t.dtype == torch.float16:
+        return KV_F16
+    raise VspecRocmError(f"{what}: need float32 or float16, got {t.dtype}")
+
+
+def paged_tree_attention(pool: PagedPool, block_tables, start_pos, q, tree_mask=None, tree_lens=None, max_start_pos=None,
+                         numerics=NUMERICS_PLAIN, scale=0.0, clamp_alpha=0.0, out=None, workspace=None, stream=None,
+                         block_used=None):
+    """vspec_rocm_paged_tree_attention: q [B][N][Hq][D] (float32 or float16, device; N drafted
+    nodes of each sequence, in slots start_pos[b] + j) -> out, as q.  tree_mask: [B][N] int64
+    (or uint64), bit j of row i lets node i see node j, None: a chain; tree_lens: [B], None: N
+    each; max_start_pos: the host's upper bound on start_pos (None: read back from the device).
+    workspace None: a temporary of torch's allocator, which also serves calls captured into a
+    graph."""
+    import torch
+
+    dev = pool.device
+    _on_device("paged_tree_attention", dev, q=q, tree_mask=tree_mask, out=out, workspace=workspace)
+    if q.dim() != 4 or not q.is_contiguous():
+        raise VspecRocmError("paged_tree_attention: q must be a contiguous [B][N][Hq][D]")
+    B, N, Hq, D = q.shape
+    bt, sp = _i32(block_tables, dev), _i32(start_pos, dev)
+    tl = None if tree_lens is None else _i32(tree_lens, dev)
+    bu = None if block_used is None else _i32(block_used, dev)
+    if D != pool.head_dim or bt.dim() != 2 or bt.shape[0] != B or sp.numel() != B or (tl is not None and tl.numel() != B):
+        raise VspecRocmError("paged_tree_attention: q, block_tables, start_pos and tree_lens do not fit together")
+    if bu is not None and bu.shape != bt.shape:
+        raise VspecRocmError("paged_tree_attention: block_used must have the shape of block_tables")
+    if tree_mask is not None and (tree_mask.dtype not in (torch.int64, torch.uint64) or tree_mask.shape != (B, N) or
+                                  not tree_mask.is_contiguous()):
+        raise VspecRocmError("paged_tree_attention: tree_mask must be a contiguous int64 [B][N]")
+    if max_start_pos is None:
+        max_start_pos = max(int(sp.max()), 0) if B else 0
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise VspecRocmError("paged_tree_attention: out must be as q")
+    d = VspecTreeAttnDesc()
+    d.kv = pool.desc()
+    d.batch, d.num_q_heads, d.num_nodes = B, Hq, N
+    d.block_tables, d.max_blocks_per_seq = bt.data_ptr(), bt.shape[1]
+    d.start_pos, d.max_start_pos = sp.data_ptr(), max_start_pos
+    d.tree_lens, d.tree_mask, d.block_used = _ptr(tl), _ptr(tree_mask), _ptr(bu)
+    d.q, d.out, d.io_dtype = q.data_ptr(), out.data_ptr(), _io_type("paged_tree_attention", q)
+    d.scale, d.numerics, d.clamp_alpha = scale, numerics, clamp_alpha
+    if workspace is None:
+        need = lib().vspec_rocm_paged_tree_attention_workspace_bytes(C.byref(d))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace is not None:
+        d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    d.stream = _stream(stream)
+    _check(lib().vspec_rocm_paged_tree_attention(C.byref(d)), "paged_tree_attention")
+    if stream is not None:
+        _hold(stream, bt, sp, tl, bu, out, workspace)
+    return out
+
+
+def pool_array(pools):
+    """The descriptors of the pools of all layers, which kv_accept takes: an engine makes them once."""
+    pools = list(pools)
+    arr = (VspecPagedKV * len(pools))(*[p.desc() for p in pools])
+    arr.pools = pools  # the tensors live as long as their addresses
+    return arr
+
+
+def kv_accept(pools, block_tables, start_pos, path, num_nodes, stream=None):
+    """vspec_rocm_kv_accept: slot start_pos[b] + i gets the row of slot start_pos[b] + path[b][i]
+    in every pool (a pool_array, or pools), up to the first entry of path [B][<= 64] outside
+    0..num_nodes-1.  Returns the new lengths, int32 [B]."""
+    import torch
+
+    if not isinstance(pools, C.Array):
+        pools = pool_array(pools)
+    if not len(pools):
+        raise VspecRocmError("kv_accept: no pools")
+    dev = pools.pools[0].device
+    _on_device("kv_accept", dev)
+    bt, sp, pa = _i32(block_tables, dev), _i32(start_pos, dev), _i32(path, dev)
+    if pa.dim() != 2 or bt.dim() != 2 or not bt.shape[0] == sp.numel() == pa.shape[0]:
+        raise VspecRocmError("kv_accept: block_tables, start_pos and path do not fit together")
+    out = torch.empty(pa.shape[0], dtype=torch.int32, device=dev)
+    _check(lib().vspec_rocm_kv_accept(pools, len(pools), pa.shape[0], bt.data_ptr(), bt.shape[1], sp.data_ptr(),
+                                      pa.data_ptr(), pa.shape[1], num_nodes, out.data_ptr(), _stream(stream)), "kv_accept")
+    if stream is not None:
+        _hold(stream, bt, sp, pa, out)
+    return out
+
+
+def rope(positions, q=None, k=None, rope_dim=None, base=10000.0, layout=ROPE_HALF, scaling=ROPE_SCALE_NONE, factor=1.0,
+         trained_len=0, low=1.0, high=4.0, magnitude=0.0, inverse=False, q_out=None, k_out=None, stream=None):
+    """vspec_rocm_rope: rows q [T][Hq][D] and k [T][Hk][D] (float32 or float16, device, any
+    token and head strides, adjacent elements; either may be None) turned by positions [T].
+    q_out / k_out: as the inputs, or the inputs themselves (in place); None: new tensors.
+    Returns (q_out, k_out)."""
+    import torch
+
+    if q is None and k is None:
+        raise VspecRocmError("rope: need q or k")
+    first = q if q is not None else k
+    _on_device("rope", first.device, q=q, k=k, q_out=q_out, k_out=k_out)
+    pos = _i32(positions, first.device)
+    T, _, D = first.shape
+    d = VspecRopeDesc()
+    d.num_tokens, d.head_dim, d.rope_dim = T, D, D if rope_dim is None else rope_dim
+    d.dtype, d.layout, d.inverse = _io_type("rope", first), layout, int(inverse)
+    d.scaling, d.trained_len, d.base, d.factor = scaling, trained_len, base, factor
+    d.low, d.high, d.magnitude = low, high, magnitude
+    d.positions = pos.data_ptr()
+    outs = []
+    for rows, x, out in ((d.q, q, q_out), (d.k, k, k_out)):
+        if x is not None:
+            if out is None:
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            for t in (x, out):
+                if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or t.dtype != first.dtype or t.stride(2) != 1:
+                    raise VspecRocmError("rope: rows must be [T][heads][D] of one type, the elements of a row adjacent")
+                if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+                    raise VspecRocmError("rope: an expanded operand (stride 0) has no rows of its own")
+            if out.shape != x.shape or pos.numel() != T:
+                raise VspecRocmError("rope: positions, q, k and their outputs do not fit together")
+            rows.in_, rows.out, rows.num_heads = x.data_ptr(), out.data_ptr(), x.shape[1]
+            rows.in_token_stride, rows.in_head_stride = x.stride(0), x.stride(1)
+            rows.out_token_stride, rows.out_head_stride = out.stride(0), out.stride(1)
+        outs.append(out)
+    d.stream = _stream(stream)
+    _check(lib().vspec_rocm_rope(C.byref(d)), "rope")
+    if stream is not None:
+        _hold(stream, pos, *outs)
+    return tuple(outs)
 
 
 def backend() -> VspecBackend:

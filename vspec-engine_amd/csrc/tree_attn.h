@@ -22,6 +22,13 @@ struct TreeParams {
     float alpha;       // std-clamp alpha
     float logit_clip;  // 24 * log2(e) in 3-bit mode, +inf otherwise
     float input_clip;  // 16 in 3-bit mode, +inf otherwise
+    // work split: an item is (sequence, kv head, group of column tiles); its steps are cut into
+    // up to `parts` parts of at least part_steps steps, a workgroup each
+    uint32_t parts, part_steps;
+    uint32_t col_groups;  // of col_waves * CT tiles of 16 columns
+    uint32_t col_waves;   // waves of a workgroup side by side over columns: 1, 2 or 4
+    float* part_acc;      // [item][part][column tile][D/16][lane][4]
+    float* part_ml;       // [item][part][column tile][16][2]: reference point (log2 units), sum
 };
 
 // A sequence's slots: [0, start) are the prefix, start + j is node j, j < len.
@@ -42,5 +49,34 @@ __device__ __forceinline__ uint64_t tree_bits(const TreeParams& p, uint32_t b, i
     const uint64_t m = p.tree_mask ? p.tree_mask[(size_t)b * p.nodes + i] : (2ull << i) - 1;
     return i < len ? m & all : 0;
 }
+
+// A sequence's steps of NT tiles: first the tiles that hold prefix alone, then those from the first
+// node's on.  Part i of them begins at step i * chunk.
+struct TreeParts {
+    int tiles, prefix_tiles, prefix_steps;
+    int steps, count, chunk;
+};
+template <int NT>
+__device__ __forceinline__ TreeParts tree_parts(const TreeParams& p, const TreeSpan& s) {
+    TreeParts r;
+    r.tiles = s.len ? (s.end + kTile - 1) / kTile : 0;  // (no nodes: nothing to read)
+    r.prefix_tiles = min(s.start / kTile, r.tiles);
+    r.prefix_steps = (r.prefix_tiles + NT - 1) / NT;
+    r.steps = r.prefix_steps + (r.tiles - r.prefix_tiles + NT - 1) / NT;
+    const int most = max(1, min((int)p.parts, (r.steps + (int)p.part_steps - 1) / (int)p.part_steps));
+    r.chunk = max(1, (r.steps + most - 1) / most);
+    r.count = max(1, (r.steps + r.chunk - 1) / r.chunk);
+    return r;
+}
+
+// Launch the kernels of one pool type and head size (tree_mfma.hip): ct column tiles a wave.
+void launch_tree_f32_d64(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+void launch_tree_f32_d128(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+void launch_tree_f16_d64(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+void launch_tree_f16_d128(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+void launch_tree_int4_d64(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+void launch_tree_int4_d128(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
+// 16-token tiles of a step
+constexpr int tree_step_tiles(int dtype) { return dtype == VSPEC_KV_F32 ? 1 : 2; }
 
 }  // namespace vkv

@@ -1,6 +1,5 @@
-// tree_attn.hip -- attention of a tree of drafted tokens over the paged cache
-// (vspec_rocm_paged_tree_attention): every node of a sequence sees the cached prefix and the
-// nodes that its mask names, in one pass over the sequence's tokens.
+// tree_attn.hip -- vspec_rocm_paged_tree_attention: its checks, its plan and its launches (the
+// kernels: tree_mfma.hip).
 #include <math.h>
 
 #include "host.h"
@@ -8,98 +7,6 @@
 
 namespace vkv {
 namespace {
-
-// Element e of the key or value row in `slot` of (block, head) bh.
-template <int DT, int D>
-__device__ __forceinline__ float key_at(const TreeParams& p, size_t bh, uint32_t slot, uint32_t e) {
-    const uint32_t P = p.block_tokens;
-    const size_t row = bh * P + slot;
-    if constexpr (DT == VSPEC_KV_F32) return reinterpret_cast<const float*>(p.k)[row * D + e];
-    if constexpr (DT == VSPEC_KV_F16) return half_bits_to_float(reinterpret_cast<const uint16_t*>(p.k)[row * D + e]);
-    return nibble((uint32_t)p.k[row * (D / 2) + e / 2], (int)(e & 1u)) *
-           half_bits_to_float(p.ks[int4_ks_index(bh, D / 32, P, slot, e / 32)]);
-}
-template <int DT, int D>
-__device__ __forceinline__ float value_at(const TreeParams& p, size_t bh, uint32_t slot, uint32_t e) {
-    const uint32_t P = p.block_tokens;
-    if constexpr (DT == VSPEC_KV_F32) return reinterpret_cast<const float*>(p.v)[(bh * P + slot) * D + e];
-    if constexpr (DT == VSPEC_KV_F16) return half_bits_to_float(reinterpret_cast<const uint16_t*>(p.v)[f16_v_index(bh, P, D, slot, e)]);
-    uint32_t high;
-    const uint8_t c = p.v[int4_v_byte(bh, P, D, slot, e, &high)];
-    return nibble((uint32_t)c, (int)high) * half_bits_to_float(p.vs[(bh * P + slot) * (D / 32) + e / 32]);
-}
-
-// One wave for each (node, query head, sequence): 64 tokens at a time, a lane each for the
-// scores, then D / 64 elements of the output a lane.
-template <int DT, int D, typename IO>
-__global__ __launch_bounds__(64) void tree_rows(TreeParams p) {
-    __shared__ float q[D];
-    __shared__ float pr[64];
-    __shared__ size_t bhs[64];
-    const uint32_t i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int lane = threadIdx.x;
-    constexpr int E = D / 64;
-    const TreeSpan sp = tree_span(p, b);
-    const size_t row = (((size_t)b * p.nodes + i) * p.hq + h) * D;
-    const uint64_t bits = tree_bits(p, b, (int)i, sp.len);
-    IO* out = reinterpret_cast<IO*>(p.out) + row;
-
-    float x[E], sum = 0.f, var = 0.f;
-    for (int e = 0; e < E; ++e) {
-        x[e] = (float)(reinterpret_cast<const IO*>(p.q) + row)[lane + 64 * e];
-        sum += x[e];
-    }
-    const float mean = wave_sum(sum) * (1.0f / D);
-    for (int e = 0; e < E; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
-    const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(wave_sum(var) * (1.0f / D))), p.input_clip);
-    for (int e = 0; e < E; ++e) q[lane + 64 * e] = fminf(fmaxf(x[e], -th), th) * p.scale;
-    __syncthreads();
-
-    float m = -INFINITY, l = 0.f, acc[E] = {};
-    const int end = (int)i < sp.len ? sp.end : 0;
-    for (int t0 = 0; t0 < end; t0 += 64) {
-        const int t = t0 + lane;
-        bool sees = t < end && (t < sp.start || (bits >> (t - sp.start) & 1));
-        float s = -INFINITY;
-        if (sees) {
-            const size_t at = (size_t)b * p.max_blocks + t / p.block_tokens;
-            const uint32_t slot = (uint32_t)t % p.block_tokens;
-            const int entry = p.block_tables[at];
-            sees = entry >= 0 && (uint32_t)entry < p.num_blocks && (!p.block_used || (int)slot < p.block_used[at]);
-            if (sees) {
-                const size_t bh = (size_t)entry * p.hkv + h / p.group;
-                bhs[lane] = bh;
-                float sm = 0.f, v2 = 0.f, dot = 0.f;
-                for (uint32_t e = 0; e < D; ++e) sm += key_at<DT, D>(p, bh, slot, e);
-                sm *= 1.0f / D;
-                for (uint32_t e = 0; e < D; ++e) {
-                    const float y = key_at<DT, D>(p, bh, slot, e) - sm;
-                    v2 = fmaf(y, y, v2);
-                }
-                const float kth = fminf(fmaxf(1e-6f, p.alpha * sqrtf(v2 * (1.0f / D))), p.input_clip);
-                for (uint32_t e = 0; e < D; ++e) dot = fmaf(q[e], fminf(fmaxf(key_at<DT, D>(p, bh, slot, e), -kth), kth), dot);
-                s = fminf(fmaxf(dot, -p.logit_clip), p.logit_clip);
-            }
-        }
-        const float mt = fmaxf(m, wave_max(s));
-        const float base = mt == -INFINITY ? 0.f : mt;
-        const float f = exp2f(m - base);
-        m = mt;
-        const float w = exp2f(s - base);
-        l = l * f + wave_sum(w);
-        pr[lane] = sees ? w : -1.f;
-        __syncthreads();
-        for (int e = 0; e < E; ++e) acc[e] *= f;
-        for (int n = 0; n < 64; ++n) {
-            if (pr[n] < 0.f) continue;
-            for (int e = 0; e < E; ++e) {
-                acc[e] = fmaf(pr[n], value_at<DT, D>(p, bhs[n], (uint32_t)(t0 + n) % p.block_tokens, lane + 64 * e), acc[e]);
-            }
-        }
-        __syncthreads();
-    }
-    for (int e = 0; e < E; ++e) out[lane + 64 * e] = (IO)(m == -INFINITY ? 0.f : acc[e] / l);
-}
 
 int check_tree(const VspecTreeAttnDesc* d) {
     if (!d) {
@@ -139,11 +46,42 @@ int check_tree(const VspecTreeAttnDesc* d) {
     return 1;
 }
 
-template <int DT, int D>
-void launch_rows(const TreeParams& p, int32_t io, hipStream_t s) {
-    const dim3 grid(p.nodes, p.hq, p.batch);
-    if (io == VSPEC_KV_F32) hipLaunchKernelGGL((tree_rows<DT, D, float>), grid, dim3(64), 0, s, p);
-    else hipLaunchKernelGGL((tree_rows<DT, D, _Float16>), grid, dim3(64), 0, s, p);
+struct TreePlan {
+    uint32_t ct, col_waves, col_groups, parts, part_steps;
+    size_t acc_floats, ws_bytes;
+};
+
+// Columns first: a wave holds up to 4 tiles of 16 columns and a workgroup up to 16, so that K and
+// V are read once for as many rows as the registers hold.  Then parts, as many as fill the card.
+TreePlan plan_tree(const VspecTreeAttnDesc* d) {
+    TreePlan pl = {};
+    const uint32_t cols = d->num_nodes * (d->num_q_heads / d->kv.num_kv_heads);
+    const uint32_t tiles = (cols + 15) / 16;
+    const uint32_t most_ct = d->kv.dtype == VSPEC_KV_F32 ? 2 : 4;
+    pl.ct = tiles == 1 ? 1 : tiles == 2 ? 2 : most_ct;
+    pl.col_waves = tiles <= most_ct ? 1 : tiles <= 2 * most_ct ? 2 : 4;
+    pl.col_groups = (tiles + pl.ct * pl.col_waves - 1) / (pl.ct * pl.col_waves);
+    const uint64_t cap = (uint64_t)d->max_blocks_per_seq * d->kv.block_tokens;
+    uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
+    if (bound > cap) bound = cap;
+    const uint32_t per = 16 * tree_step_tiles(d->kv.dtype);
+    const uint64_t steps = (bound + per - 1) / per;
+    const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups * d->batch;
+    const uint64_t slots = (uint64_t)host_num_cus() * (pl.ct == 1 ? 2 : 1);
+    uint64_t parts = items ? slots / items : 1;
+    const uint64_t most = steps * pl.col_waves / 8;  // two steps a wave
+    if (parts > most) parts = most;
+    if (parts < 1) parts = 1;
+    if (parts > 256) parts = 256;
+    pl.part_steps = (uint32_t)((steps + parts - 1) / parts);
+    if (pl.part_steps < 1) pl.part_steps = 1;
+    pl.parts = (uint32_t)parts;
+    if (parts > 1) {
+        const size_t states = (size_t)(items * parts * pl.col_waves * pl.ct);
+        pl.acc_floats = states * d->kv.head_dim * 16;
+        pl.ws_bytes = (pl.acc_floats + states * 32) * sizeof(float);
+    }
+    return pl;
 }
 
 }  // namespace
@@ -153,7 +91,7 @@ using namespace vkv;
 
 extern "C" size_t vspec_rocm_paged_tree_attention_workspace_bytes(const VspecTreeAttnDesc* desc) {
     if (!check_tree(desc)) return 0;
-    return 0;
+    return plan_tree(desc).ws_bytes;
 }
 
 extern "C" int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc) {
@@ -195,12 +133,35 @@ extern "C" int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc) {
     p.alpha = desc->clamp_alpha > 0.f ? desc->clamp_alpha : 4.5f;
     p.logit_clip = three ? 24.0f * kLog2e : INFINITY;
     p.input_clip = three ? 16.0f : INFINITY;
+    const TreePlan pl = plan_tree(desc);
+    void* ws = nullptr;
+    if (pl.ws_bytes) {
+        if (desc->workspace) {
+            if (desc->workspace_bytes < pl.ws_bytes || (uintptr_t)desc->workspace % 16 != 0) {
+                host_error("paged_tree_attention: workspace too small (%zu < %zu) or not 16-byte aligned", desc->workspace_bytes, pl.ws_bytes);
+                return 0;
+            }
+            ws = desc->workspace;
+        } else {
+            ws = host_workspace(pl.ws_bytes);
+            if (!ws) {
+                host_error("paged_tree_attention: cannot allocate %zu workspace bytes", pl.ws_bytes);
+                return 0;
+            }
+        }
+    }
+    p.parts = pl.parts;
+    p.part_steps = pl.part_steps;
+    p.col_groups = pl.col_groups;
+    p.col_waves = pl.col_waves;
+    p.part_acc = (float*)ws;
+    p.part_ml = (float*)ws + pl.acc_floats;
     hipStream_t s = (hipStream_t)desc->stream;
     const bool wide = kv.head_dim == 128;
     switch (kv.dtype) {
-        case VSPEC_KV_F32: wide ? launch_rows<VSPEC_KV_F32, 128>(p, desc->io_dtype, s) : launch_rows<VSPEC_KV_F32, 64>(p, desc->io_dtype, s); break;
-        case VSPEC_KV_F16: wide ? launch_rows<VSPEC_KV_F16, 128>(p, desc->io_dtype, s) : launch_rows<VSPEC_KV_F16, 64>(p, desc->io_dtype, s); break;
-        default: wide ? launch_rows<VSPEC_KV_INT4, 128>(p, desc->io_dtype, s) : launch_rows<VSPEC_KV_INT4, 64>(p, desc->io_dtype, s); break;
+        case VSPEC_KV_F32: (wide ? launch_tree_f32_d128 : launch_tree_f32_d64)(p, desc->io_dtype, pl.ct, s); break;
+        case VSPEC_KV_F16: (wide ? launch_tree_f16_d128 : launch_tree_f16_d64)(p, desc->io_dtype, pl.ct, s); break;
+        default: (wide ? launch_tree_int4_d128 : launch_tree_int4_d64)(p, desc->io_dtype, pl.ct, s); break;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

@@ -1,0 +1,898 @@
+// tree_mfma.hip -- attention of a drafted tree over the paged cache on the matrix cores.
+//
+// The C = nodes * group query rows that share a kv head are columns; 16 of them are a column
+// tile.  A wave holds CT column tiles and goes over its share of the tokens once, a step of 32
+// (f32 pools 16) tokens at a time, with the running maximum and sum of an online softmax:
+//   S^T[16 tok][16 col] = K[16 tok][D] x Q^T     A = K rows as loaded, B = q
+//   O^T[d][16 col]     += V^T[d][tok] x P^T      A = V as loaded, B = p, straight from the S^T
+//                                                accumulators: lane (g, n) holds tokens 4g..4g+3
+//                                                of column n in both
+// so neither scores nor weights pass through LDS.  f16 and int4 pools use 16x16x32 f16 MFMAs
+// (the 8 tokens of a lane in a step are tokens 4g..4g+3 of two tiles), f32 pools 16x16x4 f32.
+//
+// Precision.  f32 rows (IO = float) keep 22 bits of q and p, each split in two f16 (hi + lo), and
+// of int4 values; f16 rows take q, p and int4 values rounded to f16 once.  Sums are f32.  p is
+// scaled by 2^kHeadroom against the reference point of the softmax, which follows the maximum
+// only when that has grown by 2^8, so p <= 2^11 fits f16 and weights down to 2^-27 of the
+// largest count.
+//
+// The clip of every key to its own standard deviation is screened as in the decode
+// (decode_mfma.hip); the keys of a tile that it may reach are multiplied again, clipped, in two
+// f16 parts.
+//
+// Work: an item is (sequence, kv head, group of column tiles).  The waves of a workgroup are
+// col_waves side by side over columns, times 4 / col_waves over steps; items are cut into parts
+// over their steps where there are too few for the card, and a second launch joins the parts.
+#include "tree_attn.h"
+
+namespace vkv {
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+// log2 of p at the reference point: p <= 2^(kHeadroom + kThreshold) = 2^11, times 2^4 for int4 values
+// beyond one f16
+constexpr float kHeadroom = 3.0f;
+constexpr float kThreshold = 8.0f;  // growth of the maximum, log2 units, that moves the reference point
+
+__device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// A 16-token tile as loaded: lane (g, n) holds K elements of token n and V elements of tokens
+// 4g..4g+3.
+template <int DT, int D>
+struct Tile;
+template <int D>
+struct Tile<VSPEC_KV_F16, D> {
+    uint4 k[D / 32];  // d = 32i + 8g .. +7
+    uint4 v[D / 32];  // d = 32i + 2n (first 8 bytes, 4 tokens) and d + 1
+};
+template <int D>
+struct Tile<VSPEC_KV_INT4, D> {
+    uint32_t k[D / 32];       // code dwords g*D/32 + i: one group's
+    uint32_t v[D / 32];       // lane chunk (g, n)
+    uint32_t vs[D / 16];      // scales of tokens 4g..4g+3, D/32 halves each
+    uint32_t ks;              // scale of token n and the lane's group
+};
+template <int D>
+struct Tile<VSPEC_KV_F32, D> {
+    float k[D / 4];           // d = 16i + 4g .. +3
+    float v[4][D / 16];       // token 4g + r, d = 64i + 4n .. +3
+};
+
+// Output element d of accumulator register r of d-tile j in lanes of row group g.
+template <int DT>
+__device__ __forceinline__ int out_dim(int j, int g, int r) {
+    if constexpr (DT == VSPEC_KV_F16) return 32 * (j / 2) + 8 * g + 2 * r + j % 2;
+    if constexpr (DT == VSPEC_KV_INT4) return 16 * j + 4 * g + r;
+    return 64 * (j / 4) + 16 * g + 4 * r + j % 4;
+}
+
+// int4 codes to f16: pairs (nibble k, nibble k + 4) of a dword, exact (a nibble in the mantissa under
+// a magic exponent, minus its bias)
+__device__ __forceinline__ void codes_to_f16(uint32_t w, h2_t out[4]) {
+    const uint32_t w8 = w >> 8;
+    const h2_t b0 = {(_Float16)1032.0f, (_Float16)1032.0f}, b1 = {(_Float16)72.0f, (_Float16)72.0f};
+    out[0] = __builtin_bit_cast(h2_t, ((w ^ 0x00080008u) & 0x000F000Fu) | 0x64006400u) - b0;
+    out[1] = __builtin_bit_cast(h2_t, ((w ^ 0x00800080u) & 0x00F000F0u) | 0x54005400u) - b1;
+    out[2] = __builtin_bit_cast(h2_t, ((w8 ^ 0x00080008u) & 0x000F000Fu) | 0x64006400u) - b0;
+    out[3] = __builtin_bit_cast(h2_t, ((w8 ^ 0x00800080u) & 0x00F000F0u) | 0x54005400u) - b1;
+}
+
+// Between matrix instructions and the first vector instruction that reads their results.  Left to
+// itself hipcc 7.2 mixes the two across branches, and one accumulator register of a tile then lost
+// part of its sum (rows 4g of every second tile, off by 2^-13; seen in a kernel that added two chains
+// behind a branch).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <bool B>
+struct BoolTag {
+    static constexpr bool value = B;
+};
+
+constexpr uint32_t kBigScale = 0x6C00u;  // 2^12: a code times it may pass f16's range
+
+// fp16 scales of group c of the lane's tokens 4g + 2e and 4g + 2e + 1 (token r's halves start at word r NQ / 2)
+template <int NQ, typename T>
+__device__ __forceinline__ uint32_t int4_scale_pair(const T& t, int c, int e) {
+    const uint32_t w0 = t.vs[(2 * e) * NQ / 2 + c / 2], w1 = t.vs[(2 * e + 1) * NQ / 2 + c / 2];
+    return c % 2 ? (w0 >> 16) | (w1 & 0xffff0000u) : (w0 & 0xffffu) | (w1 << 16);
+}
+// Values of d-tiles 2c (e) and 2c + 1 (o) from a code dword of group c: rounded, and with LOW the exact rest
+template <bool LOW>
+__device__ __forceinline__ void int4_values(uint32_t codes, const h2_t (&scale)[2], h4_t& e, h4_t& o, h4_t& el, h4_t& ol) {
+    h2_t q[4];  // tokens 0, 1 of e and of o, tokens 2, 3 of e and of o
+    codes_to_f16(codes, q);
+    const h2_t e0 = q[0] * scale[0], e1 = q[2] * scale[1], o0 = q[1] * scale[0], o1 = q[3] * scale[1];
+    e = __builtin_shufflevector(e0, e1, 0, 1, 2, 3);
+    o = __builtin_shufflevector(o0, o1, 0, 1, 2, 3);
+    if constexpr (LOW) {
+        el = __builtin_shufflevector(__builtin_elementwise_fma(q[0], scale[0], -e0), __builtin_elementwise_fma(q[2], scale[1], -e1), 0, 1, 2, 3);
+        ol = __builtin_shufflevector(__builtin_elementwise_fma(q[1], scale[0], -o0), __builtin_elementwise_fma(q[3], scale[1], -o1), 0, 1, 2, 3);
+    }
+}
+
+template <int DT, int D, typename IO, int CT>
+__global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
+    constexpr bool F32 = DT == VSPEC_KV_F32;
+    constexpr bool SPLIT = sizeof(IO) == 4 && !F32;      // q and p in two f16 parts
+    constexpr bool VLO = SPLIT && DT == VSPEC_KV_INT4;   // K and V in two f16 parts
+    constexpr int NT = tree_step_tiles(DT);
+    constexpr int NQ = D / 32;   // f16 score MFMAs of a tile
+    constexpr int NDT = D / 16;  // d-tiles of the output
+    typedef Tile<DT, D> T;
+    __shared__ uint64_t bits_sh[64];
+    __shared__ f4_t red[4][NDT][64];
+    __shared__ float red_ml[4][16][2];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int token_waves = 4 / (int)p.col_waves;
+    const int cw = wave / token_waves, tw = wave - cw * token_waves;
+
+    const uint32_t b = blockIdx.y;
+    const uint32_t item = blockIdx.x / p.parts, part = blockIdx.x - item * p.parts;
+    const uint32_t h = item / p.col_groups, cg = item - h * p.col_groups;
+    const TreeSpan sp = tree_span(p, b);
+    const TreeParts tp = tree_parts<NT>(p, sp);
+    if ((int)part >= tp.count) return;
+    const int lo = (int)part * tp.chunk, hi = min(lo + tp.chunk, tp.steps);
+
+    if (threadIdx.x < p.nodes) bits_sh[threadIdx.x] = tree_bits(p, b, threadIdx.x, sp.len);
+    __syncthreads();
+
+    const int P = (int)p.block_tokens;
+    const int tiles_per_block = P / kTile;
+
+    // ---- tiles ----
+    // Loads go out whatever the entry (one that names no block reads block 0) and hold as many
+    // valid tokens as the call returns.
+    auto load_tile = [&](const int tile, const bool in, T& f) -> int {
+        const size_t row = (size_t)b * p.max_blocks + (in ? tile / tiles_per_block : 0);
+        const int entry = as_const(p.block_tables)[row];
+        const bool ok = in && entry >= 0 && (uint32_t)entry < p.num_blocks;
+        const size_t bh = (size_t)(ok ? entry : 0) * p.hkv + h;
+        const int slot0 = in ? (tile % tiles_per_block) * kTile : 0;
+        if constexpr (DT == VSPEC_KV_F16) {
+            const uint4* kr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(p.k) + (bh * P + slot0 + n) * D + 8 * g);
+            const uint4* vr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(p.v) + f16_v_index(bh, P, D, slot0 + 4 * g, 2 * n));
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) f.k[i] = kr[4 * i];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) f.v[i] = vr[16 * i];
+        } else if constexpr (DT == VSPEC_KV_INT4) {
+            const uint32_t* kr = reinterpret_cast<const uint32_t*>(p.k + (bh * P + slot0 + n) * (D / 2)) + g * NQ;
+            const uint32_t* vr = reinterpret_cast<const uint32_t*>(p.v + bh * ((size_t)P * D / 2) + (size_t)slot0 * (D / 2)) + (16 * g + n) * NQ;
+            const uint32_t* vs = reinterpret_cast<const uint32_t*>(p.vs + (bh * P + slot0 + 4 * g) * NQ);
+            if constexpr (NQ == 4) {
+                const uint4 a = *reinterpret_cast<const uint4*>(kr), c = *reinterpret_cast<const uint4*>(vr);
+                const uint4 s0 = reinterpret_cast<const uint4*>(vs)[0], s1 = reinterpret_cast<const uint4*>(vs)[1];
+                f.k[0] = a.x, f.k[1] = a.y, f.k[2] = a.z, f.k[3] = a.w;
+                f.v[0] = c.x, f.v[1] = c.y, f.v[2] = c.z, f.v[3] = c.w;
+                f.vs[0] = s0.x, f.vs[1] = s0.y, f.vs[2] = s0.z, f.vs[3] = s0.w;
+                f.vs[4] = s1.x, f.vs[5] = s1.y, f.vs[6] = s1.z, f.vs[7] = s1.w;
+            } else {
+                const uint2 a = *reinterpret_cast<const uint2*>(kr), c = *reinterpret_cast<const uint2*>(vr);
+                const uint4 s0 = *reinterpret_cast<const uint4*>(vs);
+                f.k[0] = a.x, f.k[1] = a.y;
+                f.v[0] = c.x, f.v[1] = c.y;
+                f.vs[0] = s0.x, f.vs[1] = s0.y, f.vs[2] = s0.z, f.vs[3] = s0.w;
+            }
+            f.ks = p.ks[int4_ks_index(bh, NQ, P, slot0 + n, (uint32_t)(g * NQ) / 4u)];
+        } else {
+            const float* kr = reinterpret_cast<const float*>(p.k) + (bh * P + slot0 + n) * D + 4 * g;
+            const float* vr = reinterpret_cast<const float*>(p.v) + (bh * P + slot0 + 4 * g) * D + 4 * n;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const float4 w = *reinterpret_cast<const float4*>(kr + 16 * i);
+                f.k[4 * i] = w.x, f.k[4 * i + 1] = w.y, f.k[4 * i + 2] = w.z, f.k[4 * i + 3] = w.w;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const float4 w = *reinterpret_cast<const float4*>(vr + (size_t)r * D + 64 * i);
+                    f.v[r][4 * i] = w.x, f.v[r][4 * i + 1] = w.y, f.v[r][4 * i + 2] = w.z, f.v[r][4 * i + 3] = w.w;
+                }
+            }
+        }
+        int cap = ok ? kTile : 0;
+        if (p.block_used) cap = ok ? used_cap(as_const(p.block_used)[row], slot0) : 0;
+        return min(cap, max(sp.end - tile * kTile, 0));
+    };
+    struct Step {
+        T t[NT];
+        int valid[NT];
+        int tile;  // the first one
+    };
+    // prefix steps hold whole tiles of the prefix, tree steps those from the first that holds a node
+    auto load = [&](int step, const int limit, Step& s) {
+        step = __builtin_amdgcn_readfirstlane(step);
+        const bool prefix = step < tp.prefix_steps;
+        s.tile = prefix ? step * NT : tp.prefix_tiles + (step - tp.prefix_steps) * NT;
+        const int last = prefix ? tp.prefix_tiles : tp.tiles;
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            const bool in = step < limit && s.tile + a < last;
+            s.valid[a] = load_tile(s.tile + a, in, s.t[a]);
+            if (!in) s.valid[a] = 0;
+        }
+    };
+
+    // this wave's prefix steps and its tree steps (which come first: their loads share the round trip)
+    Step ring[2];
+    const int prefix_hi = min(hi, tp.prefix_steps);
+    int step = lo + tw;
+    int tree_step = step >= tp.prefix_steps ? step : step + (tp.prefix_steps - step + token_waves - 1) / token_waves * token_waves;
+    const bool has_tree = tree_step < hi;
+    if (has_tree) load(tree_step, hi, ring[1]);
+    load(step, prefix_hi, ring[0]);
+
+    // ---- q: columns of this wave ----
+    // Column c is node c / group, head c % group of the kv head's.  The operands hold clip(q) 2^e
+    // (e != 0 only for f32 rows outside f16's range, qnorm_shift); scores come out in that unit
+    // and fac takes them to log2 units.
+    const int cols = (int)(p.nodes * p.group);
+    const int ctile0 = ((int)cg * (int)p.col_waves + cw) * CT;
+    h8_t qh[F32 ? 1 : CT][NQ], ql[SPLIT ? CT : 1][NQ];
+    float qf[F32 ? CT : 1][F32 ? D / 4 : 1];
+    float fac[CT];
+    int node[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int c = (ctile0 + ct) * 16 + n;
+        const int i = c / (int)p.group;
+        node[ct] = min(i, (int)p.nodes - 1);
+        const bool live = c < cols && i < sp.len;
+        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live ? i : 0)) * p.hq + (size_t)h * p.group + (live ? c - i * (int)p.group : 0)) * D;
+        constexpr int E = D / 4;
+        float x[E];
+#pragma unroll
+        for (int u = 0; u < E / 4; ++u) {
+            // four adjacent elements: of the lane's 8 of k-step u / 2 (f16: 32i + 8g, int4: 8 (g NQ + i)), or f32's 16u + 4g
+            const int d = F32 ? 16 * u + 4 * g : (DT == VSPEC_KV_F16 ? 32 * (u / 2) + 8 * g : 8 * (g * NQ + u / 2)) + 4 * (u % 2);
+            if constexpr (sizeof(IO) == 4) {
+                const float4 w = *reinterpret_cast<const float4*>(src + d);
+                x[4 * u] = w.x, x[4 * u + 1] = w.y, x[4 * u + 2] = w.z, x[4 * u + 3] = w.w;
+            } else {
+                const h4_t w = *reinterpret_cast<const h4_t*>(src + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * u + e] = (float)w[e];
+            }
+        }
+        float sum = 0.f, var = 0.f, am = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = live ? x[e] : 0.f;
+            sum += x[e];
+        }
+        sum = add_rows(sum);
+        const float mean = sum * (1.0f / D);
+#pragma unroll
+        for (int e = 0; e < E; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
+        const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = fminf(fmaxf(x[e], -th), th);
+            am = fmaxf(am, fabsf(x[e]));
+        }
+        int ex = 0;
+        if constexpr (SPLIT) ex = qnorm_shift(max_rows(am));
+        fac[ct] = sum != sum ? sum : p.scale * pow2i(-ex);  // (a row with NaN gives NaN: the clips would hide it)
+        const float up = pow2i(ex);
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) qf[ct][e] = x[e];
+        } else {
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    // int4: halves 2m, 2m + 1 are nibbles m, m + 4
+                    const float y = x[8 * k + (DT == VSPEC_KV_INT4 ? e / 2 + 4 * (e % 2) : e)] * up;
+                    const _Float16 hi16 = (_Float16)y;
+                    qh[ct][k][e] = hi16;
+                    if constexpr (SPLIT) ql[ct][k][e] = (_Float16)(y - (float)hi16);
+                }
+            }
+        }
+    }
+
+    // ---- state of every column: reference point mf (log2 units), the score that moves it, sum, output ----
+    f4_t acc[CT][NDT];
+    float limit[CT], mf[CT], l[CT];
+    float clip[CT];  // of scores
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        limit[ct] = -INFINITY;
+        clip[ct] = p.logit_clip / fac[ct];
+        mf[ct] = -1e30f;
+        l[ct] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NDT; ++j) acc[ct][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto process = [&](auto tree_tag, Step& s) {
+        constexpr bool TREE = decltype(tree_tag)::value;
+        // ---- K operands, each key held to its own limit ----
+        h8_t kh[F32 ? 1 : NT][NQ], kl[SPLIT ? NT : 1][NQ];
+        bool low[NT];    // kl holds something
+        float kunit[NT]; // scores come out divided by this
+        bool nans[NT];   // a key may be NaN
+#pragma unroll
+        for (int a = 0; a < NT; ++a) {
+            T& t = s.t[a];
+            low[a] = VLO;
+            kunit[a] = 1.f;
+            nans[a] = F32;
+            if constexpr (F32) {
+                // two passes over the row in registers, and the clip itself
+                float sum = 0.f, var = 0.f;
+#pragma unroll
+                for (int e = 0; e < D / 4; ++e) sum += t.k[e];
+                const float mean = add_rows(sum) * (1.0f / D);
+#pragma unroll
+                for (int e = 0; e < D / 4; ++e) var = fmaf(t.k[e] - mean, t.k[e] - mean, var);
+                const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+#pragma unroll
+                for (int e = 0; e < D / 4; ++e) t.k[e] = t.k[e] != t.k[e] ? t.k[e] : __builtin_amdgcn_fmed3f(t.k[e], -th, th);
+            } else {
+                float s1 = 0.f, s2 = 0.f, mx;
+                bool large = false;
+                if constexpr (DT == VSPEC_KV_F16) {
+                    const h2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+                    h2_t mx2 = {(_Float16)0.f, (_Float16)0.f};
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        kh[a][i] = __builtin_bit_cast(h8_t, t.k[i]);
+                        const uint32_t w4[4] = {t.k[i].x, t.k[i].y, t.k[i].z, t.k[i].w};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const h2_t y = __builtin_bit_cast(h2_t, w4[c]);
+                            s1 = __builtin_amdgcn_fdot2(y, ones, s1, false);
+                            s2 = __builtin_amdgcn_fdot2(y, y, s2, false);
+                            mx2 = __builtin_elementwise_max(mx2, __builtin_elementwise_abs(y));
+                        }
+                    }
+                    mx = fmaxf((float)mx2[0], (float)mx2[1]);
+                } else {
+                    const float sc = half_bits_to_float(t.ks);
+                    // a code times a scale past 7500 may pass f16's range: the tile's scales drop by 2^4
+                    large = __builtin_amdgcn_ballot_w64(n < s.valid[a] && fabsf(sc) > 7500.f) != 0;
+                    _Float16 s16 = __builtin_bit_cast(_Float16, (uint16_t)t.ks);
+                    if (large) {
+                        s16 *= (_Float16)0.0625f;
+                        kunit[a] = 16.f;
+                    }
+                    const h2_t s2v = {s16, s16};
+                    int c1 = 0, c2 = 0;
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        c1 = __builtin_amdgcn_sdot8((int)t.k[i], 0x11111111, c1, false);
+                        c2 = __builtin_amdgcn_sdot8((int)t.k[i], (int)t.k[i], c2, false);
+                        h2_t q4[4];
+                        codes_to_f16(t.k[i], q4);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const h2_t y = q4[c] * s2v;
+                            kh[a][i][2 * c] = y[0];
+                            kh[a][i][2 * c + 1] = y[1];
+                            if constexpr (VLO) {
+                                const h2_t z = __builtin_elementwise_fma(q4[c], s2v, -y);  // exact
+                                kl[a][i][2 * c] = z[0];
+                                kl[a][i][2 * c + 1] = z[1];
+                            }
+                        }
+                    }
+                    s1 = sc * (float)c1;
+                    s2 = sc * sc * (float)c2;
+                    mx = 8.0f * fabsf(sc);
+                }
+                s1 = add_rows(s1);
+                s2 = add_rows(s2);
+                const float mean1 = s1 * (1.0f / D), ex2 = s2 * (1.0f / D);
+                const float var1 = ex2 - mean1 * mean1;
+                const float th1 = fminf(fmaxf(1e-6f, p.alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), p.input_clip);
+                // the margins of the decode's screen; !(<=) also takes what is not finite
+                const bool flag = !(mx <= th1 * (1.0f - 0.0009765625f)) || var1 <= ex2 * 0.0009765625f;
+                const uint64_t any = __builtin_amdgcn_ballot_w64(flag && n < s.valid[a]);
+                if (any != 0) {
+                    // the flagged keys (any lane of token n flags it), exactly: two-pass deviation, and the clipped row
+                    // in two f16 parts.  Elements inside the limit stay exact, the limit keeps 22 bits or 2^-25.
+                    nans[a] = true;
+                    low[a] = SPLIT;
+                    const bool mine = ((any | (any >> 16) | (any >> 32) | (any >> 48)) >> n) & 1u;
+                    float x[8 * NQ], sum = 0.f, var = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        if constexpr (DT == VSPEC_KV_F16) {
+                            const h8_t w = __builtin_bit_cast(h8_t, t.k[i]);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[8 * i + e] = (float)w[e];
+                        } else {
+                            h2_t q4[4];
+                            codes_to_f16(t.k[i], q4);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[8 * i + e] = (float)q4[e / 2][e % 2] * half_bits_to_float(t.ks);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum += x[8 * i + e];
+                    }
+                    const float mean = add_rows(sum) * (1.0f / D);
+#pragma unroll
+                    for (int e = 0; e < 8 * NQ; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
+                    const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+                    const float down = large ? 0.0625f : 1.f;
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float y = x[8 * i + e];
+                            y = (y != y ? y : __builtin_amdgcn_fmed3f(y, -th, th)) * down;
+                            const _Float16 y16 = (_Float16)y;
+                            kh[a][i][e] = mine ? y16 : kh[a][i][e];
+                            if constexpr (SPLIT) {
+                                const _Float16 z16 = (_Float16)(y - (float)y16);
+                                kl[a][i][e] = mine ? z16 : VLO ? kl[a][i][e] : (_Float16)0.f;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- scores ----
+        f4_t sc[CT][NT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                f4_t c = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < D / 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(s.t[a].k[e], qf[ct][e], c, 0, 0, 0);
+                } else {
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[a][i], ql[ct][i], c, 0, 0, 0);
+                    }
+                    if constexpr (VLO) {
+#pragma unroll
+                        for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[a][i], qh[ct][i], c, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[a][i], qh[ct][i], c, 0, 0, 0);
+                }
+                sc[ct][a] = c;
+            }
+        }
+        if constexpr (SPLIT && !VLO) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                if (!low[a]) continue;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) sc[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[a][i], qh[ct][i], sc[ct][a], 0, 0, 0);
+                }
+            }
+        }
+        settle();
+        if constexpr (DT == VSPEC_KV_INT4) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int a = 0; a < NT; ++a) sc[ct][a] *= kunit[a];
+            }
+        }
+
+        // ---- softmax of column n over the lane's tokens ----
+        uint32_t sees[TREE ? CT : 1][NT];  // bit r: the lane's token r is visible to its column
+        float top[CT];
+        bool grown = false;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            top[ct] = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                f4_t x = sc[ct][a];
+                if (nans[a]) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = x[r] != x[r] ? x[r] : __builtin_amdgcn_fmed3f(x[r], -clip[ct], clip[ct]);
+                } else {
+                    // (a key with NaN is always flagged; the median would hide it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_fmed3f(x[r], -clip[ct], clip[ct]);
+                }
+                if (TREE || s.valid[a] < kTile) {
+                    uint32_t seen = 15u;
+                    if constexpr (TREE) {
+                        const int j0 = (s.tile + a) * kTile + 4 * g - sp.start;  // the node that the lane's first token is
+                        const uint64_t mine = bits_sh[node[ct]];
+                        seen = j0 <= -4 ? 15u
+                               : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
+                               : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
+                    }
+                    const int held = s.valid[a] - 4 * g;
+                    seen &= held >= 4 ? 15u : held > 0 ? (1u << held) - 1u : 0u;
+                    if constexpr (TREE) sees[ct][a] = seen;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = (seen >> r) & 1u ? x[r] : -INFINITY;
+                }
+                sc[ct][a] = x;
+                top[ct] = fmaxf(top[ct], fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+            }
+            grown = grown || top[ct] > limit[ct];
+        }
+        if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+            settle();  // (the outputs of the step before)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const float mt = max_rows(top[ct]);
+                const bool need = mt > limit[ct];
+                const float nf = fmaf(mt, fac[ct], -kHeadroom);
+                const float f = need ? __builtin_amdgcn_exp2f(mf[ct] - nf) : 1.0f;
+                limit[ct] = need ? mt + kThreshold / fac[ct] : limit[ct];
+                mf[ct] = need ? nf : mf[ct];
+                l[ct] *= f;
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) acc[ct][j] *= f;
+            }
+        }
+        h8_t ph[F32 ? 1 : CT], pl[SPLIT ? CT : 1];
+        float pf[F32 ? CT : 1][4];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int e = 0; e < 4 * NT; ++e) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[ct][e / 4][e % 4], fac[ct], -mf[ct]));
+                l[ct] += w;
+                if constexpr (F32) {
+                    pf[ct][e] = w;
+                } else {
+                    const _Float16 w16 = (_Float16)w;
+                    ph[ct][e] = w16;
+                    if constexpr (SPLIT) pl[ct][e] = (_Float16)(w - (float)w16);
+                }
+            }
+        }
+
+        // ---- V operands, O^T += V^T P^T ----
+        // Slots without a token may hold any bits and become zeros.  In tiles that hold nodes so do values
+        // that are not finite: in the products 0 * inf would reach the rows that do not see them.
+        bool wild[NT];
+        if constexpr (F32) {
+            wild[0] = false;
+            float v[4][NDT];
+            bool mine = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool held = 4 * g + r < s.valid[0];
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) {
+                    v[r][j] = s.t[0].v[r][j];
+                    if constexpr (TREE) {
+                        const bool out = !(fabsf(v[r][j]) < INFINITY);
+                        mine = mine || (held && out);
+                        v[r][j] = held && !out ? v[r][j] : 0.f;
+                    }
+                }
+            }
+            if constexpr (TREE) {
+                wild[0] = __builtin_amdgcn_ballot_w64(mine) != 0;
+            } else if (s.valid[0] < kTile) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                    for (int j = 0; j < NDT; ++j) v[r][j] = 4 * g + r < s.valid[0] ? v[r][j] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][j], pf[ct][r], acc[ct][j], 0, 0, 0);
+                }
+            }
+        } else {
+            h4_t vh[NT][NDT], vl[VLO ? NT : 1][NDT];
+            bool big = false;
+            if constexpr (DT == VSPEC_KV_INT4) {
+                bool mine_big = false;
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+                    bool mine = false;
+#pragma unroll
+                    for (int c = 0; c < NQ; ++c) {
+                        h2_t sp2[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            // in the products of scales of 2^12 and more a code may pass f16's range: they are left
+                            // for a product of their own
+                            uint32_t w = int4_scale_pair<NQ>(s.t[a], c, e);
+                            if (s.valid[a] < kTile) {
+                                w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
+                            }
+                            const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
+                            mine_big = mine_big || max(lo16, hi16) >= kBigScale;
+                            mine = mine || max(lo16, hi16) >= 0x7C00u;
+                            w &= (lo16 < kBigScale ? 0xffffu : 0u) | (hi16 < kBigScale ? 0xffff0000u : 0u);
+                            sp2[e] = __builtin_bit_cast(h2_t, w);
+                        }
+                        int4_values<VLO>(s.t[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
+                    }
+                    wild[a] = TREE && __builtin_amdgcn_ballot_w64(mine) != 0;
+                }
+                big = __builtin_amdgcn_ballot_w64(mine_big) != 0;
+            } else {
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+                    wild[a] = false;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        vh[a][2 * i] = __builtin_bit_cast(h4_t, make_uint2(s.t[a].v[i].x, s.t[a].v[i].y));
+                        vh[a][2 * i + 1] = __builtin_bit_cast(h4_t, make_uint2(s.t[a].v[i].z, s.t[a].v[i].w));
+                    }
+                    if (TREE || s.valid[a] < kTile) {
+                        bool mine = false;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool held = 4 * g + r < s.valid[a];
+#pragma unroll
+                            for (int j = 0; j < NDT; ++j) {
+                                const bool out = TREE && !(fabsf((float)vh[a][j][r]) < INFINITY);
+                                mine = mine || (held && out);
+                                vh[a][j][r] = held && !out ? vh[a][j][r] : (_Float16)0.f;
+                            }
+                        }
+                        wild[a] = __builtin_amdgcn_ballot_w64(mine) != 0;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NDT; ++j) {
+                const h8_t v = join(vh[0][j], vh[NT - 1][j]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct], acc[ct][j], 0, 0, 0);
+                    if constexpr (SPLIT) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct], acc[ct][j], 0, 0, 0);
+                    if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph[ct], acc[ct][j], 0, 0, 0);
+                }
+            }
+            if constexpr (DT == VSPEC_KV_INT4) {
+                if (big) {
+                    // the large values over 2^4 times p 2^4 (p <= 2^11)
+                    const h2_t down = {(_Float16)0.0625f, (_Float16)0.0625f};
+#pragma unroll
+                    for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                        for (int c = 0; c < NQ; ++c) {
+                            h2_t sp2[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t w = int4_scale_pair<NQ>(s.t[a], c, e);
+                                if (s.valid[a] < kTile) {
+                                    w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
+                                }
+                                const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
+                                const bool l_in = lo16 >= kBigScale && (!TREE || lo16 < 0x7C00u), h_in = hi16 >= kBigScale && (!TREE || hi16 < 0x7C00u);
+                                w &= (l_in ? 0xffffu : 0u) | (h_in ? 0xffff0000u : 0u);
+                                sp2[e] = __builtin_bit_cast(h2_t, w) * down;
+                            }
+                            int4_values<VLO>(s.t[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
+                        }
+                    }
+                    const _Float16 up = (_Float16)16.f;
+                    const h8_t up8 = {up, up, up, up, up, up, up, up};
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        const h8_t ph16 = ph[ct] * up8;
+#pragma unroll
+                        for (int j = 0; j < NDT; ++j) {
+                            const h8_t v = join(vh[0][j], vh[NT - 1][j]);
+                            acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph16, acc[ct][j], 0, 0, 0);
+                            if constexpr (SPLIT) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct] * up8, acc[ct][j], 0, 0, 0);
+                            if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph16, acc[ct][j], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        }
+        if constexpr (TREE) {
+            // What is not finite reaches the rows that see it: +inf where a visible value is +inf or NaN,
+            // and -inf where one is -inf or NaN (both: NaN), counted by products of ones.
+#pragma unroll
+            for (int a = 0; a < NT; ++a) {
+                if (!wild[a]) continue;
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) {
+                    h4_t plus, minus;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float v;
+                        if constexpr (F32) {
+                            v = s.t[a].v[r][j];
+                        } else if constexpr (DT == VSPEC_KV_F16) {
+                            const uint4 w = s.t[a].v[j / 2];
+                            const uint32_t half2 = j % 2 ? (r < 2 ? w.z : w.w) : (r < 2 ? w.x : w.y);
+                            v = half_bits_to_float((half2 >> (16 * (r % 2))) & 0xffffu);
+                        } else {
+                            const uint32_t sc16 = int4_scale_pair<NQ>(s.t[a], j / 2, r / 2) >> (16 * (r % 2)) & 0xffffu;
+                            h2_t q4[4];
+                            codes_to_f16(s.t[a].v[j / 2], q4);
+                            v = (sc16 & 0x7fffu) >= 0x7C00u ? (float)q4[j % 2 + 2 * (r / 2)][r % 2] * half_bits_to_float(sc16) : 0.f;
+                        }
+                        const bool held = 4 * g + r < s.valid[a];
+                        plus[r] = held && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                        minus[r] = held && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                    }
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        h4_t vis;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) vis[r] = (sees[ct][a] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
+                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                        const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
+                        const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
+                        settle();
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
+                            acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    if (has_tree) {
+        for (;;) {
+            process(BoolTag<true>{}, ring[1]);
+            tree_step += token_waves;
+            if (tree_step >= hi) break;
+            load(tree_step, hi, ring[1]);
+        }
+    }
+    for (; step < prefix_hi; step += 2 * token_waves) {
+        load(step + token_waves, prefix_hi, ring[1]);
+        process(BoolTag<false>{}, ring[0]);
+        load(step + 2 * token_waves, prefix_hi, ring[0]);
+        process(BoolTag<false>{}, ring[1]);
+    }
+
+    settle();
+
+    // ---- join the token waves; the output, or the part's state ----
+    const bool whole = tp.count == 1;
+    const int tiles = (int)p.col_waves * CT;
+    const size_t slot = ((size_t)b * (p.hkv * p.col_groups) + item) * p.parts + part;
+    auto finish = [&](const int ct, const int j, f4_t a, const float sum, const float ref) {
+        const int tile = cw * CT + ct;
+        if (!whole) {
+            reinterpret_cast<f4_t*>(p.part_acc)[((slot * tiles + tile) * NDT + j) * 64 + lane] = a;
+            if (j == 0 && g == 0) {
+                float* ml = p.part_ml + ((slot * tiles + tile) * 16 + n) * 2;
+                ml[0] = ref;
+                ml[1] = sum;
+            }
+            return;
+        }
+        const int c = (ctile0 + ct) * 16 + n;
+        if (c >= cols) return;
+        const int i = c / (int)p.group;
+        IO* dst = reinterpret_cast<IO*>(p.out) + (((size_t)b * p.nodes + i) * p.hq + (size_t)h * p.group + (c - i * (int)p.group)) * D;
+        const bool empty = i >= sp.len || sum == 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : a[r] / sum);
+    };
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const float sum = add_rows(l[ct]);
+        if (token_waves == 1) {
+#pragma unroll
+            for (int j = 0; j < NDT; ++j) finish(ct, j, acc[ct][j], sum, mf[ct]);
+            continue;
+        }
+        if (ct) __syncthreads();
+        if (g == 0) {
+            red_ml[wave][n][0] = mf[ct];
+            red_ml[wave][n][1] = sum;
+        }
+        __syncthreads();
+        float top = -INFINITY, total = 0.f;
+        for (int t = 0; t < token_waves; ++t) top = fmaxf(top, red_ml[cw * token_waves + t][n][0]);
+        for (int t = 0; t < token_waves; ++t) {
+            const float* ml = red_ml[cw * token_waves + t][n];
+            total += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
+        }
+        const float f = __builtin_amdgcn_exp2f(mf[ct] - top);
+#pragma unroll
+        for (int j = 0; j < NDT; ++j) red[wave][j][lane] = acc[ct][j] * f;
+        __syncthreads();
+        for (int j = tw; j < NDT; j += token_waves) {
+            f4_t a = {0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < token_waves; ++t) a += red[cw * token_waves + t][j][lane];
+            finish(ct, j, a, total, top);
+        }
+    }
+}
+
+// The parts of one column tile of an item.
+template <int DT, int D, typename IO>
+__global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t ct) {
+    constexpr int NT = tree_step_tiles(DT);
+    constexpr int NDT = D / 16;
+    const uint32_t tiles = p.col_waves * ct;
+    const uint32_t b = blockIdx.y, item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
+    const uint32_t h = item / p.col_groups, cg = item - h * p.col_groups;
+    const TreeSpan sp = tree_span(p, b);
+    const TreeParts tp = tree_parts<NT>(p, sp);
+    if (tp.count == 1) return;
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int c = (int)((cg * tiles + tile) * 16) + n;
+    const bool live = c < (int)(p.nodes * p.group);
+    const int i = c / (int)p.group;
+    const size_t slot0 = ((size_t)b * (p.hkv * p.col_groups) + item) * p.parts;
+    float top = -INFINITY, total = 0.f;
+    for (int t = 0; t < tp.count; ++t) top = fmaxf(top, p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2]);
+    for (int t = 0; t < tp.count; ++t) {
+        const float* ml = p.part_ml + (((slot0 + t) * tiles + tile) * 16 + n) * 2;
+        total += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
+    }
+    const bool empty = i >= sp.len || total == 0.f;
+    for (int j = (int)(threadIdx.x >> 6); j < NDT; j += 4) {
+        f4_t a = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < tp.count; ++t) {
+            const float f = __builtin_amdgcn_exp2f(p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2] - top);
+            a += reinterpret_cast<const f4_t*>(p.part_acc)[(((slot0 + t) * tiles + tile) * NDT + j) * 64 + lane] * f;
+        }
+        if (!live) continue;
+        IO* dst = reinterpret_cast<IO*>(p.out) + (((size_t)b * p.nodes + i) * p.hq + (size_t)h * p.group + (c - i * (int)p.group)) * D;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : a[r] / total);
+    }
+}
+
+template <int DT, int D, typename IO>
+void launch(const TreeParams& p, uint32_t ct, hipStream_t s) {
+    const dim3 grid(p.hkv * p.col_groups * p.parts, p.batch);
+    switch (ct) {
+        case 1: hipLaunchKernelGGL((tree_attention<DT, D, IO, 1>), grid, dim3(256), 0, s, p); break;
+        case 2: hipLaunchKernelGGL((tree_attention<DT, D, IO, 2>), grid, dim3(256), 0, s, p); break;
+        default:
+            if constexpr (DT != VSPEC_KV_F32) hipLaunchKernelGGL((tree_attention<DT, D, IO, 4>), grid, dim3(256), 0, s, p);
+            break;
+    }
+    if (p.parts > 1) {
+        hipLaunchKernelGGL((tree_merge<DT, D, IO>), dim3(p.hkv * p.col_groups * p.col_waves * ct, p.batch), dim3(256), 0, s, p, ct);
+    }
+}
+
+}  // namespace
+
+#define TREE_LAUNCH_(name, dt, d)                                                      \
+    void name(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s) {           \
+        if (io == VSPEC_KV_F32) launch<dt, d, float>(p, ct, s);                        \
+        else launch<dt, d, _Float16>(p, ct, s);                                        \
+    }
+#if VSPEC_HEAD_DIM == 64
+TREE_LAUNCH_(launch_tree_f32_d64, VSPEC_KV_F32, 64)
+TREE_LAUNCH_(launch_tree_f16_d64, VSPEC_KV_F16, 64)
+TREE_LAUNCH_(launch_tree_int4_d64, VSPEC_KV_INT4, 64)
+#else
+TREE_LAUNCH_(launch_tree_f32_d128, VSPEC_KV_F32, 128)
+TREE_LAUNCH_(launch_tree_f16_d128, VSPEC_KV_F16, 128)
+TREE_LAUNCH_(launch_tree_int4_d128, VSPEC_KV_INT4, 128)
+#endif
+#undef TREE_LAUNCH_
+
+}  // namespace vkv

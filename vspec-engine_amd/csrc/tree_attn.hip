@@ -48,6 +48,7 @@ int check_tree(const VspecTreeAttnDesc* d) {
 
 struct TreePlan {
     uint32_t ct, col_waves, col_groups, parts, part_steps;
+    bool wide;  // tree_wide.hip
     size_t acc_floats, ws_bytes;
 };
 
@@ -57,9 +58,14 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     TreePlan pl = {};
     const uint32_t cols = d->num_nodes * (d->num_q_heads / d->kv.num_kv_heads);
     const uint32_t tiles = (cols + 15) / 16;
-    const uint32_t most_ct = d->kv.dtype == VSPEC_KV_F32 ? 2 : 4;
-    pl.ct = tiles == 1 ? 1 : tiles == 2 ? 2 : most_ct;
-    pl.col_waves = tiles <= most_ct ? 1 : tiles <= 2 * most_ct ? 2 : 4;
+    pl.wide = d->kv.dtype != VSPEC_KV_F32 && tiles > 2;
+    if (pl.wide) {
+        pl.ct = tiles <= 4 ? 1 : 2;
+        pl.col_waves = tiles <= 8 ? 4 : 8;
+    } else {
+        pl.ct = tiles == 1 ? 1 : 2;
+        pl.col_waves = tiles <= 2 ? 1 : tiles <= 4 ? 2 : 4;
+    }
     pl.col_groups = (tiles + pl.ct * pl.col_waves - 1) / (pl.ct * pl.col_waves);
     const uint64_t cap = (uint64_t)d->max_blocks_per_seq * d->kv.block_tokens;
     uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
@@ -67,9 +73,9 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     const uint32_t per = 16 * tree_step_tiles(d->kv.dtype);
     const uint64_t steps = (bound + per - 1) / per;
     const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups * d->batch;
-    const uint64_t slots = (uint64_t)host_num_cus() * (pl.ct == 1 ? 2 : 1);
+    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : pl.ct == 1 && d->io_dtype == VSPEC_KV_F16 ? 3 : 2) : 1);
     uint64_t parts = items ? slots / items : 1;
-    const uint64_t most = steps * pl.col_waves / 8;  // two steps a wave
+    const uint64_t most = pl.wide ? steps / 4 : steps * pl.col_waves / 8;  // two steps a wave
     if (parts > most) parts = most;
     if (parts < 1) parts = 1;
     if (parts > 256) parts = 256;
@@ -129,6 +135,9 @@ extern "C" int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc) {
     p.block_tokens = kv.block_tokens;
     p.max_blocks = desc->max_blocks_per_seq;
     p.num_blocks = kv.num_blocks;
+    const uint32_t block_tiles = kv.block_tokens / kTile;
+    while ((1u << p.block_shift) < block_tiles) ++p.block_shift;
+    p.block_magic = (uint32_t)((((1ull << (27 + p.block_shift)) + block_tiles - 1) / block_tiles) << 4);
     p.scale = scale * kLog2e;
     p.alpha = desc->clamp_alpha > 0.f ? desc->clamp_alpha : 4.5f;
     p.logit_clip = three ? 24.0f * kLog2e : INFINITY;
@@ -157,11 +166,17 @@ extern "C" int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc) {
     p.part_acc = (float*)ws;
     p.part_ml = (float*)ws + pl.acc_floats;
     hipStream_t s = (hipStream_t)desc->stream;
-    const bool wide = kv.head_dim == 128;
+    const bool d128 = kv.head_dim == 128;
     switch (kv.dtype) {
-        case VSPEC_KV_F32: (wide ? launch_tree_f32_d128 : launch_tree_f32_d64)(p, desc->io_dtype, pl.ct, s); break;
-        case VSPEC_KV_F16: (wide ? launch_tree_f16_d128 : launch_tree_f16_d64)(p, desc->io_dtype, pl.ct, s); break;
-        default: (wide ? launch_tree_int4_d128 : launch_tree_int4_d64)(p, desc->io_dtype, pl.ct, s); break;
+        case VSPEC_KV_F32: (d128 ? launch_tree_f32_d128 : launch_tree_f32_d64)(p, desc->io_dtype, pl.ct, s); break;
+        case VSPEC_KV_F16:
+            if (pl.wide) (d128 ? launch_tree_wide_f16_d128 : launch_tree_wide_f16_d64)(p, desc->io_dtype, pl.ct, s);
+            else (d128 ? launch_tree_f16_d128 : launch_tree_f16_d64)(p, desc->io_dtype, pl.ct, s);
+            break;
+        default:
+            if (pl.wide) (d128 ? launch_tree_wide_int4_d128 : launch_tree_wide_int4_d64)(p, desc->io_dtype, pl.ct, s);
+            else (d128 ? launch_tree_int4_d128 : launch_tree_int4_d64)(p, desc->io_dtype, pl.ct, s);
+            break;
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

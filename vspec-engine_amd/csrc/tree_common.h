@@ -1,0 +1,118 @@
+// tree_common.h -- what the kernels of the attention of a drafted tree share: tree_mfma.hip
+// (few columns, and f32 pools) and tree_wide.hip (many columns).
+#pragma once
+#include "tree_attn.h"
+
+namespace vkv {
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+// log2 of p at the reference point: p <= 2^(kHeadroom + kThreshold) = 2^11, times 2^4 for int4 values
+// beyond one f16
+constexpr float kHeadroom = 3.0f;
+constexpr float kThreshold = 8.0f;  // growth of the maximum, log2 units, that moves the reference point
+
+__device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Output element d of accumulator register r of d-tile j in lanes of row group g.
+template <int DT>
+__device__ __forceinline__ int out_dim(int j, int g, int r) {
+    if constexpr (DT == VSPEC_KV_F16) return 32 * (j / 2) + 8 * g + 2 * r + j % 2;
+    if constexpr (DT == VSPEC_KV_INT4) return 16 * j + 4 * g + r;
+    return 64 * (j / 4) + 16 * g + 4 * r + j % 4;
+}
+
+// int4 codes to f16: pairs (nibble k, nibble k + 4) of a dword, exact (a nibble in the mantissa under
+// a magic exponent, minus its bias)
+__device__ __forceinline__ void codes_to_f16(uint32_t w, h2_t out[4]) {
+    const uint32_t w8 = w >> 8;
+    const h2_t b0 = {(_Float16)1032.0f, (_Float16)1032.0f}, b1 = {(_Float16)72.0f, (_Float16)72.0f};
+    out[0] = __builtin_bit_cast(h2_t, ((w ^ 0x00080008u) & 0x000F000Fu) | 0x64006400u) - b0;
+    out[1] = __builtin_bit_cast(h2_t, ((w ^ 0x00800080u) & 0x00F000F0u) | 0x54005400u) - b1;
+    out[2] = __builtin_bit_cast(h2_t, ((w8 ^ 0x00080008u) & 0x000F000Fu) | 0x64006400u) - b0;
+    out[3] = __builtin_bit_cast(h2_t, ((w8 ^ 0x00800080u) & 0x00F000F0u) | 0x54005400u) - b1;
+}
+
+// Between matrix instructions and the first vector instruction that reads their results.  Left to
+// itself hipcc 7.2 mixes the two across branches, and one accumulator register of a tile then lost
+// part of its sum (rows 4g of every second tile, off by 2^-13; seen in a kernel that added two chains
+// behind a branch).
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <bool B>
+struct BoolTag {
+    static constexpr bool value = B;
+};
+
+constexpr uint32_t kBigScale = 0x6C00u;  // 2^12: a code times it may pass f16's range
+
+// fp16 scales of group c of the lane's tokens 4g + 2e and 4g + 2e + 1 (token r's halves start at word r NQ / 2)
+template <int NQ, typename T>
+__device__ __forceinline__ uint32_t int4_scale_pair(const T& t, int c, int e) {
+    const uint32_t w0 = t.vs[(2 * e) * NQ / 2 + c / 2], w1 = t.vs[(2 * e + 1) * NQ / 2 + c / 2];
+    return c % 2 ? (w0 >> 16) | (w1 & 0xffff0000u) : (w0 & 0xffffu) | (w1 << 16);
+}
+// Values of d-tiles 2c (e) and 2c + 1 (o) from a code dword of group c: rounded, and with LOW the exact rest
+template <bool LOW>
+__device__ __forceinline__ void int4_values(uint32_t codes, const h2_t (&scale)[2], h4_t& e, h4_t& o, h4_t& el, h4_t& ol) {
+    h2_t q[4];  // tokens 0, 1 of e and of o, tokens 2, 3 of e and of o
+    codes_to_f16(codes, q);
+    const h2_t e0 = q[0] * scale[0], e1 = q[2] * scale[1], o0 = q[1] * scale[0], o1 = q[3] * scale[1];
+    e = __builtin_shufflevector(e0, e1, 0, 1, 2, 3);
+    o = __builtin_shufflevector(o0, o1, 0, 1, 2, 3);
+    if constexpr (LOW) {
+        el = __builtin_shufflevector(__builtin_elementwise_fma(q[0], scale[0], -e0), __builtin_elementwise_fma(q[2], scale[1], -e1), 0, 1, 2, 3);
+        ol = __builtin_shufflevector(__builtin_elementwise_fma(q[1], scale[0], -o0), __builtin_elementwise_fma(q[3], scale[1], -o1), 0, 1, 2, 3);
+    }
+}
+
+// The parts of one column tile of an item.
+template <int DT, int D, typename IO>
+__global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t tiles) {
+    constexpr int NT = tree_step_tiles(DT);
+    constexpr int NDT = D / 16;
+    const uint32_t b = blockIdx.y, item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
+    const uint32_t h = item / p.col_groups, cg = item - h * p.col_groups;
+    const TreeSpan sp = tree_span(p, b);
+    const TreeParts tp = tree_parts<NT>(p, sp);
+    if (tp.count == 1) return;
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int c = (int)((cg * tiles + tile) * 16) + n;
+    const bool live = c < (int)(p.nodes * p.group);
+    const int i = c / (int)p.group;
+    const size_t slot0 = ((size_t)b * (p.hkv * p.col_groups) + item) * p.parts;
+    float top = -INFINITY, total = 0.f;
+    for (int t = 0; t < tp.count; ++t) top = fmaxf(top, p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2]);
+    for (int t = 0; t < tp.count; ++t) {
+        const float* ml = p.part_ml + (((slot0 + t) * tiles + tile) * 16 + n) * 2;
+        total += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
+    }
+    const bool empty = i >= sp.len || total == 0.f;
+    for (int j = (int)(threadIdx.x >> 6); j < NDT; j += 4) {
+        f4_t a = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < tp.count; ++t) {
+            const float f = __builtin_amdgcn_exp2f(p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2] - top);
+            a += reinterpret_cast<const f4_t*>(p.part_acc)[(((slot0 + t) * tiles + tile) * NDT + j) * 64 + lane] * f;
+        }
+        if (!live) continue;
+        IO* dst = reinterpret_cast<IO*>(p.out) + (((size_t)b * p.nodes + i) * p.hq + (size_t)h * p.group + (c - i * (int)p.group)) * D;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : a[r] / total);
+    }
+}
+
+template <int DT, int D, typename IO>
+void launch_merge(const TreeParams& p, uint32_t tiles, hipStream_t s) {
+    hipLaunchKernelGGL((tree_merge<DT, D, IO>), dim3(p.hkv * p.col_groups * tiles, p.batch), dim3(256), 0, s, p, tiles);
+}
+
+}  // namespace
+}  // namespace vkv

@@ -1,0 +1,785 @@
+// tree_wide.hip -- attention of a drafted tree over f16 and int4 pools where many query rows share
+// a kv head (more than 32: nodes times GQA group).
+//
+// The products are those of tree_mfma.hip, S^T = K Q^T and O^T += V^T P^T with 16 columns to a
+// tile, but here the W waves of a workgroup are side by side over the columns, CT tiles each, and
+// share every K and V tile through LDS in the order in which the matrix instructions take it.
+// What is done to a key or value once for all columns is done once by the workgroup:
+//   f16   tiles stream into an LDS ring (buffer loads straight into LDS, DEPTH steps).  The wave
+//         that loaded a key's row screens it for the clip to its own standard deviation, rewrites a
+//         clipped row in place and leaves its low part beside it.
+//   int4  codes and scales stream into a ring of each wave; it turns its share of a step into f16
+//         rows (and their low parts, for f32 queries) in LDS, clipped on the way.
+// A wave's column then costs per 32 tokens its matrix instructions, 8 weights a lane and 16 reads
+// of 16 bytes from LDS.  With CT = 2 and 8 waves the LDS reads (128 KB a step, 1024 cycles) are as
+// long as the f16 matrix work of 256 columns; with one tile a wave they would be twice that.
+//
+// One barrier a step orders the ring (f16): a wave issues the loads of step s + DEPTH - 1 into the
+// slot of step s - 1, which every wave left before the last barrier.
+#include "tree_common.h"
+
+namespace vkv {
+namespace {
+
+// A descriptor in scalar registers, from values that every lane holds alike
+__device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes) {
+    const rsrc_t r = tile_rsrc(base, bytes);
+    return rsrc_t{__builtin_amdgcn_readfirstlane(r[0]), __builtin_amdgcn_readfirstlane(r[1]), __builtin_amdgcn_readfirstlane(r[2]),
+                  __builtin_amdgcn_readfirstlane(r[3])};
+}
+
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <typename IO>
+constexpr bool SPLIT_IO = sizeof(IO) == 4;
+
+template <int DT, int D, typename IO, int CT, int W>
+__global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree_wide(TreeParams p) {
+    constexpr bool F16 = DT == VSPEC_KV_F16;
+    constexpr bool SPLIT = sizeof(IO) == 4;   // q and p in two f16 parts
+    constexpr bool VLO = SPLIT && !F16;       // K and V in two f16 parts
+    constexpr int NQ = D / 32, NDT = D / 16;
+    constexpr int CPT = D / 8;                // 8-element chunks of a row
+    constexpr int TI = 64 / CPT;              // rows that a wave takes at a time, a chunk a lane
+    constexpr int SETS = W == 4 && D == 128 ? 2 : 1;
+    constexpr int TPO = TI * SETS;            // rows of a step that a wave looks after: TPO w ..
+    constexpr int OWNERS = 32 / TPO;          // waves that look after rows
+    constexpr int CL = 16 / TI;
+    constexpr int kTileB = 32 * D;            // bytes of a tile in f16
+    constexpr int kStageB = 4 * kTileB;       // K of both tiles, V of both
+    constexpr int DEPTH = F16 ? (W == 8 ? 4 : 3) : 1;
+    constexpr int RAW = 4;                    // steps of codes in the ring
+    constexpr int kRawB = F16 ? 16 : 512 * SETS + 512;  // of a wave and step: K, V, K scales, V scales
+    __shared__ __align__(16) uint8_t stage[DEPTH * kStageB];
+    __shared__ __align__(16) uint8_t low[SPLIT ? (F16 ? 2 * 2 * kTileB : kStageB) : 16];  // low parts: f16 [slot][K], int4 as a stage
+    __shared__ __align__(16) uint8_t raw[F16 ? 16 : RAW * OWNERS * kRawB];
+    // a bit for each row of a step, TPO to the byte of its wave: clipped or not finite; K (int4) and V (int4)
+    // hold a 16th of the value; V held something that is not finite
+    __shared__ __align__(8) uint8_t marks[2][4][8];
+    __shared__ uint64_t bits_sh[64];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const uint32_t b = blockIdx.y;
+    const uint32_t item = (uint32_t)uniform((int)(blockIdx.x / p.parts)), part = blockIdx.x - item * p.parts;
+    const uint32_t h = (uint32_t)uniform((int)(item / p.col_groups)), cg = item - h * p.col_groups;
+    const TreeSpan sp = tree_span(p, b);
+    const TreeParts tp = tree_parts<2>(p, sp);
+    if ((int)part >= tp.count) return;
+    const int lo = (int)part * tp.chunk, hi = min(lo + tp.chunk, tp.steps);
+    if (threadIdx.x < 64) bits_sh[threadIdx.x] = threadIdx.x < p.nodes ? tree_bits(p, b, threadIdx.x, sp.len) : 0;
+
+    const int P = (int)own_scalar(p.block_tokens);
+    const int32_t* const tables = own_scalar(p.block_tables + (size_t)b * p.max_blocks);
+    const int32_t* const used = own_scalar(p.block_used ? p.block_used + (size_t)b * p.max_blocks : nullptr);
+    const uint8_t* const kdata = own_scalar(p.k);
+    const uint8_t* const vdata = own_scalar(p.v);
+    const uint16_t* const kscales = own_scalar(p.ks);
+    const uint16_t* const vscales = own_scalar(p.vs);
+    const uint32_t num_blocks = own_scalar(p.num_blocks), hkv = own_scalar(p.hkv);
+    const uint32_t magic = own_scalar(p.block_magic), shift = own_scalar(p.block_shift);
+    const float alpha = own_scalar(p.alpha), input_clip = own_scalar(p.input_clip);
+
+    // Steps ahead of the one at work: their table entries are read a step before their loads go out, and how
+    // many tokens their tiles hold stays in scalar registers until they are worked on.
+    struct Entries {
+        int block[2], used[2];
+    };
+    auto first_tile = [&](const int step) { return step < tp.prefix_steps ? 2 * step : tp.prefix_tiles + 2 * (step - tp.prefix_steps); };
+    auto last_tile = [&](const int step) { return step < tp.prefix_steps ? tp.prefix_tiles : tp.tiles; };
+    auto fetch = [&](int step) -> Entries {
+        step = __builtin_amdgcn_readfirstlane(step);
+        Entries e;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const int tile = first_tile(step) + a;
+            const bool in = step < hi && tile < last_tile(step);
+            const int row = in ? tree_block_of(magic, shift, tile) : 0;
+            const int entry = as_const(tables)[row];
+            e.block[a] = in && entry >= 0 && (uint32_t)entry < num_blocks ? entry : -1;
+            e.used[a] = used ? as_const(used)[row] : P;
+        }
+        return e;
+    };
+    // where tile a of a step lies, and how many tokens it holds (0: it is not read)
+    struct Where {
+        size_t bh;
+        int slot0, valid;
+    };
+    auto where = [&](const int step, const int a, const Entries& e) -> Where {
+        const int tile = first_tile(step) + a;
+        const bool ok = e.block[a] >= 0;
+        Where w;
+        w.bh = (size_t)(ok ? e.block[a] : 0) * hkv + h;
+        w.slot0 = ok ? tile * kTile - tree_block_of(magic, shift, tile) * P : 0;
+        w.valid = ok ? min(min(kTile, sp.end - tile * kTile), max(0, e.used[a] - w.slot0)) : 0;
+        return w;
+    };
+
+    // ---- loads of this wave's share of a step ----
+    const bool owner = wave < OWNERS;
+    const int my_tile = (TPO * wave) / kTile & 1;    // the tile of its rows
+    const int my_part = (TPO * wave) % kTile / TPO;  // and which TPO rows of it
+    uint32_t koff[SETS], voff[SETS];                 // f16: byte offsets of this lane's chunks in the tile
+    if constexpr (F16) {
+#pragma unroll
+        for (int k = 0; k < SETS; ++k) {
+            // rows TI m .. of the tile.  Lane (position) l of the 1 KB holds chunk c of row t such that the 16 rows
+            // of one chunk lie in different banks
+            const int m = my_part * SETS + k, t = lane % TI;
+            const int c = CL * (lane / 16) + (((lane % 16) / TI) ^ m);
+            koff[k] = (uint32_t)((TI * m + t) * 2 * D + 16 * c);
+            voff[k] = (uint32_t)(g * 8 * D + (32 * m + 2 * n) * 8);  // V operands m of the tile
+        }
+    }
+    const uint32_t stage0 = lds_addr(stage), raw0 = lds_addr(raw);
+    auto load = [&](const Where& w, const int slot) {
+        if (!owner) return;
+        if constexpr (F16) {
+            const uint32_t bytes = w.valid > 0 ? kTileB : 0;
+            const size_t at = (w.bh * P + w.slot0) * (size_t)(2 * D);
+            const rsrc_t kr = uniform_rsrc(kdata + at, bytes), vr = uniform_rsrc(vdata + at, bytes);
+            const uint32_t dst = stage0 + slot * kStageB + my_tile * kTileB + my_part * SETS * 1024;
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) lds_load16(__builtin_amdgcn_readfirstlane(dst + 1024 * k), kr, koff[k]);
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) lds_load16(__builtin_amdgcn_readfirstlane(dst + 2 * kTileB + 1024 * k), vr, voff[k]);
+        } else {
+            const uint32_t bytes = w.valid > 0 ? 8 * D : 0;
+            const size_t at = (w.bh * P + w.slot0) * (size_t)(D / 2);
+            const rsrc_t kr = uniform_rsrc(kdata + at, bytes), vr = uniform_rsrc(vdata + at, bytes);
+            const rsrc_t ksr = uniform_rsrc(kscales + w.bh * NQ * P + w.slot0, w.valid > 0 ? (uint32_t)((NQ - 1) * P * 2 + 32) : 0u);
+            const rsrc_t vsr = uniform_rsrc(vscales + (w.bh * P + w.slot0) * NQ, w.valid > 0 ? 32 * NQ : 0);
+            const uint32_t dst = raw0 + (slot * OWNERS + wave) * kRawB;
+            const uint32_t from = my_part * TPO * (D / 2) + 4 * lane;
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                lds_load4(__builtin_amdgcn_readfirstlane(dst + 256 * k), kr, from + 256 * k);
+                lds_load4(__builtin_amdgcn_readfirstlane(dst + 256 * (SETS + k)), vr, from + 256 * k);
+            }
+            lds_load4(__builtin_amdgcn_readfirstlane(dst + 512 * SETS), ksr, lane < 8 * NQ ? (uint32_t)((lane / 8) * P * 2 + (lane % 8) * 4) : 0x7fffffffu);
+            lds_load4(__builtin_amdgcn_readfirstlane(dst + 512 * SETS + 256), vsr, 4 * lane);
+        }
+    };
+    constexpr int kLoads = F16 ? 2 * SETS : 2 * SETS + 2;  // of a step
+
+    // ---- what a wave does to its rows of a step before all waves read them ----
+    // sum over the lanes that hold a row: f16 lanes with the same lane % TI, int4 CPT adjacent ones
+    auto row_sum = [&](float x) {
+        if constexpr (F16) {
+            x += row_dpp<kRowRor8>(x);
+            if constexpr (TI == 4) x += row_dpp<kRowRor4>(x);
+            return add_rows(x);
+        } else {
+            return group_sum<CPT>(x);
+        }
+    };
+    // the bits of its rows (of set k) from a ballot in which any lane of a row speaks for it
+    auto row_bits = [&](uint64_t m) -> uint32_t {
+        if constexpr (F16) {
+            m |= m >> 32;
+            m |= m >> 16;
+            m |= m >> 8;
+            if constexpr (TI == 4) m |= m >> 4;
+            return (uint32_t)m & ((1u << TI) - 1u);
+        } else {
+            uint32_t r = 0;
+#pragma unroll
+            for (int t = 0; t < TI; ++t) r |= (uint32_t)((m >> (CPT * t)) & ((1ull << CPT) - 1)) ? 1u << t : 0u;
+            return r;
+        }
+    };
+    auto limit_of = [&](float var) { return fminf(fmaxf(1e-6f, alpha * sqrtf(var * (1.0f / D))), input_clip); };
+    auto prepare = [&](const int step, const int valid, const int slot, const int mark, const int raw_slot) {
+        if (!owner) return;
+        uint32_t clipped = 0, kbig = 0, vbig = 0, wild = 0;
+        // V of slots without a token may hold any bits and becomes zeros.  In tiles that hold nodes so does
+        // what is not finite: in the products 0 * inf would reach the rows that do not see it
+        const bool tree = (first_tile(step) + my_tile) * kTile + valid > sp.start;
+        if constexpr (F16) {
+            uint8_t* mine = stage + slot * kStageB + my_tile * kTileB + my_part * SETS * 1024 + 16 * lane;
+            const h2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(mine + 1024 * k);
+                const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+                float s1 = 0.f, s2 = 0.f;
+                h2_t mx2 = {(_Float16)0.f, (_Float16)0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const h2_t y = __builtin_bit_cast(h2_t, w4[c]);
+                    s1 = __builtin_amdgcn_fdot2(y, ones, s1, false);
+                    s2 = __builtin_amdgcn_fdot2(y, y, s2, false);
+                    mx2 = __builtin_elementwise_max(mx2, __builtin_elementwise_abs(y));
+                }
+                const float mx = fmaxf((float)mx2[0], (float)mx2[1]);
+                const float mean1 = row_sum(s1) * (1.0f / D), ex2 = row_sum(s2) * (1.0f / D);
+                const float var1 = ex2 - mean1 * mean1;
+                const float th1 = fminf(fmaxf(1e-6f, alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), input_clip);
+                // the margins of the decode's screen; !(<=) also takes what is not finite
+                const bool flag = !(mx <= th1 * (1.0f - 0.0009765625f)) || var1 <= ex2 * 0.0009765625f;
+                const int row = TI * (my_part * SETS + k) + lane % TI;
+                const uint64_t any = __builtin_amdgcn_ballot_w64(flag && row < valid);
+                if (any == 0) continue;
+                // exactly, for the rows that it takes: two-pass deviation, the clipped row in two f16 parts.
+                // Elements inside the limit stay exact, the limit keeps 22 bits or 2^-25.
+                const uint32_t rows = row_bits(any);
+                clipped |= rows << (TI * k);
+                const h8_t x8 = __builtin_bit_cast(h8_t, w);
+                float x[8], sum = 0.f, var = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = (float)x8[e];
+                    sum += x[e];
+                }
+                const float mean = row_sum(sum) * (1.0f / D);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
+                const float th = limit_of(row_sum(var));
+                h8_t yh, yl;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = x[e] != x[e] ? x[e] : __builtin_amdgcn_fmed3f(x[e], -th, th);
+                    yh[e] = (_Float16)y;
+                    yl[e] = (_Float16)(y - (float)yh[e]);
+                }
+                if ((rows >> (lane % TI)) & 1u) {
+                    *reinterpret_cast<h8_t*>(mine + 1024 * k) = yh;
+                    if constexpr (SPLIT) *reinterpret_cast<h8_t*>(low + mark * 2 * kTileB + my_tile * kTileB + (my_part * SETS + k) * 1024 + 16 * lane) = yl;
+                }
+            }
+            if (tree || valid < kTile) {
+#pragma unroll
+                for (int k = 0; k < SETS; ++k) {
+                    h8_t* at = reinterpret_cast<h8_t*>(mine + 2 * kTileB + 1024 * k);
+                    h8_t v = *at;
+                    bool out = false;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const bool held = 4 * g + e % 4 < valid;
+                        const bool odd = tree && held && !(fabsf((float)v[e]) < INFINITY);
+                        out = out || odd;
+                        v[e] = held && !odd ? v[e] : (_Float16)0.f;
+                    }
+                    *at = v;
+                    wild |= __builtin_amdgcn_ballot_w64(out) != 0 ? 1u : 0u;
+                }
+            }
+        } else {
+            const uint8_t* mine = raw + (raw_slot * OWNERS + wave) * kRawB;
+            const uint16_t* kscale = reinterpret_cast<const uint16_t*>(mine + 512 * SETS);
+            const uint16_t* vscale = reinterpret_cast<const uint16_t*>(mine + 512 * SETS + 256);
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                const int row = my_part * TPO + TI * k + lane / CPT, c = lane % CPT;  // row of the tile, chunk
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(mine + 256 * k + 4 * lane);
+                uint16_t s16 = kscale[(c / 4) * 16 + row];
+                const float sc = half_bits_to_float(s16);
+                const int c1 = __builtin_amdgcn_sdot8((int)w, 0x11111111, 0, false);
+                const int c2 = __builtin_amdgcn_sdot8((int)w, (int)w, 0, false);
+                const float mean1 = row_sum(sc * (float)c1) * (1.0f / D), ex2 = row_sum(sc * sc * (float)c2) * (1.0f / D);
+                const float var1 = ex2 - mean1 * mean1;
+                const float th1 = fminf(fmaxf(1e-6f, alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), input_clip);
+                const float mx = 8.0f * fabsf(sc);
+                // (a code times a scale past 7500 may pass f16's range)
+                const bool flag = !(mx <= th1 * (1.0f - 0.0009765625f)) || var1 <= ex2 * 0.0009765625f || mx > 60000.f;
+                h2_t q4[4];
+                codes_to_f16(w, q4);
+                h8_t yh, yl;
+                const h2_t s2v = {__builtin_bit_cast(_Float16, s16), __builtin_bit_cast(_Float16, s16)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const h2_t y = q4[e] * s2v;
+                    yh[2 * e] = y[0], yh[2 * e + 1] = y[1];
+                    if constexpr (VLO) {
+                        const h2_t z = __builtin_elementwise_fma(q4[e], s2v, -y);  // exact
+                        yl[2 * e] = z[0], yl[2 * e + 1] = z[1];
+                    }
+                }
+                const uint64_t any = __builtin_amdgcn_ballot_w64(flag && row < valid);
+                if (any != 0) {
+                    const uint32_t rows = row_bits(any);
+                    clipped |= rows << (TI * k);
+                    const uint32_t large = row_bits(__builtin_amdgcn_ballot_w64(mx > 60000.f && row < valid));
+                    kbig |= large << (TI * k);
+                    float x[8], sum = 0.f, var = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = (float)q4[e / 2][e % 2] * sc;
+                        sum += x[e];
+                    }
+                    const float mean = row_sum(sum) * (1.0f / D);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
+                    const float th = limit_of(row_sum(var));
+                    const float down = (large >> (lane / CPT)) & 1u ? 0.0625f : 1.f;
+                    const bool mine_too = (rows >> (lane / CPT)) & 1u;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = (x[e] != x[e] ? x[e] : __builtin_amdgcn_fmed3f(x[e], -th, th)) * down;
+                        const _Float16 y16 = (_Float16)y, z16 = (_Float16)(y - (float)y16);
+                        yh[e] = mine_too ? y16 : yh[e];
+                        if constexpr (VLO) yl[e] = mine_too ? z16 : yl[e];
+                    }
+                }
+                const int m = row / TI, t = row % TI;
+                const int at = my_tile * kTileB + m * 1024 + (16 * (c / CL) + ((c % CL) ^ m) * TI + t) * 16;
+                *reinterpret_cast<h8_t*>(stage + at) = yh;
+                if constexpr (VLO) *reinterpret_cast<h8_t*>(low + at) = yl;
+            }
+#pragma unroll
+            for (int k = 0; k < SETS; ++k) {
+                // V: word c of lane chunk (vg, vn) of the tile, tokens 4 vg .. 4 vg + 3
+                const int idx = my_part * (TPO * D / 8) + 64 * k + lane;
+                const int c = idx % NQ, chunk = idx / NQ, vg = chunk / 16;
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(mine + 256 * (SETS + k) + 4 * lane);
+                uint32_t sw[2], top = 0;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t a = vscale[(4 * vg + 2 * e) * NQ + c], z = vscale[(4 * vg + 2 * e + 1) * NQ + c];
+                    a = 4 * vg + 2 * e < valid ? a : 0u;
+                    z = 4 * vg + 2 * e + 1 < valid ? z : 0u;
+                    top = max(top, max(a & 0x7fffu, z & 0x7fffu));
+                    sw[e] = a | (z << 16);
+                }
+                if (tree && __builtin_amdgcn_ballot_w64(top >= 0x7C00u) != 0) {
+                    wild = 1;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        sw[e] &= ((sw[e] & 0x7fffu) < 0x7C00u ? 0xffffu : 0u) | (((sw[e] >> 16) & 0x7fffu) < 0x7C00u ? 0xffff0000u : 0u);
+                    }
+                }
+                h2_t sp2[2] = {__builtin_bit_cast(h2_t, sw[0]), __builtin_bit_cast(h2_t, sw[1])};
+                if (__builtin_amdgcn_ballot_w64(top >= kBigScale) != 0) {
+                    // tokens with a scale that large in any group: a 16th of the value, 16 times the weight
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        uint32_t most = (sw[r / 2] >> (16 * (r % 2))) & 0x7fffu;
+                        most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+                        if constexpr (NQ == 4) most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+                        const bool is = most >= kBigScale;
+                        sp2[r / 2][r % 2] *= is ? (_Float16)0.0625f : (_Float16)1.f;
+                        const uint64_t all = __builtin_amdgcn_ballot_w64(is);
+                        // the wave's V words belong to TPO tokens, 4 for each row group in it
+                        if constexpr (NQ == 4) vbig |= all ? 1u << (4 * k + r) : 0u;
+                        else vbig |= ((uint32_t)all ? 1u << r : 0u) | ((uint32_t)(all >> 32) ? 16u << r : 0u);
+                    }
+                }
+                h4_t ve, vo, vel, vol;
+                int4_values<VLO>(w, sp2, ve, vo, vel, vol);
+                const int at = 2 * kTileB + my_tile * kTileB + c * 1024 + (chunk % 64) * 16;
+                *reinterpret_cast<h8_t*>(stage + at) = join(ve, vo);
+                if constexpr (VLO) *reinterpret_cast<h8_t*>(low + at) = join(vel, vol);
+            }
+        }
+        if (lane == 0) {
+            marks[mark][0][wave] = (uint8_t)clipped;
+            marks[mark][1][wave] = (uint8_t)kbig;
+            marks[mark][2][wave] = (uint8_t)vbig;
+            marks[mark][3][wave] = (uint8_t)wild;
+        }
+    };
+    // the marks of tile a: bit mark_bit(n) of the word speaks for its token n
+    auto mark_word = [&](const int mark, const int which, const int a) -> uint32_t {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&marks[mark][which][TPO == 4 ? 4 * a : 0]);
+        return __builtin_amdgcn_readfirstlane(TPO == 4 ? w : (w >> (16 * a)) & 0xffffu);
+    };
+    auto mark_bit = [](int t) { return TPO == 4 ? 8 * (t >> 2) + (t & 3) : t; };
+
+    // ---- the first steps on their way, then q ----
+    constexpr int AHEAD = F16 ? DEPTH - 1 : RAW - 1;
+    int held[AHEAD + 1];  // tokens of the tiles (second: 256 times) of the step at work and of those on their way
+    auto load_step = [&](int step, const int slot, const Entries& e) -> int {
+        step = __builtin_amdgcn_readfirstlane(step);
+        const Where w0 = where(step, 0, e), w1 = where(step, 1, e);
+        load({my_tile ? w1.bh : w0.bh, my_tile ? w1.slot0 : w0.slot0, my_tile ? w1.valid : w0.valid}, slot);
+        return w0.valid | (w1.valid << 8);
+    };
+    Entries ahead = fetch(lo);
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+        const Entries e = ahead;
+        ahead = fetch(lo + s + 1);
+        held[s] = load_step(lo + s, s, e);
+    }
+
+    const int cols = (int)(p.nodes * p.group);
+    const int ctile0 = ((int)cg * W + wave) * CT;
+    h8_t qh[CT][NQ], ql[SPLIT ? CT : 1][NQ];
+    float fac[CT];
+    int node[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int c = (ctile0 + ct) * 16 + n;
+        const int i = c / (int)p.group;
+        node[ct] = min(i, (int)p.nodes - 1);
+        const bool live = c < cols && i < sp.len;
+        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live ? i : 0)) * p.hq + (size_t)h * p.group + (live ? c - i * (int)p.group : 0)) * D;
+        float x[8 * NQ], sum = 0.f, var = 0.f, am = 0.f;
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) {
+            if constexpr (SPLIT) {
+                const float4 w0 = *reinterpret_cast<const float4*>(src + 32 * k + 8 * g), w1 = *reinterpret_cast<const float4*>(src + 32 * k + 8 * g + 4);
+                x[8 * k] = w0.x, x[8 * k + 1] = w0.y, x[8 * k + 2] = w0.z, x[8 * k + 3] = w0.w;
+                x[8 * k + 4] = w1.x, x[8 * k + 5] = w1.y, x[8 * k + 6] = w1.z, x[8 * k + 7] = w1.w;
+            } else {
+                const h8_t w = *reinterpret_cast<const h8_t*>(src + 32 * k + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[8 * k + e] = (float)w[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8 * NQ; ++e) {
+            x[e] = live ? x[e] : 0.f;
+            sum += x[e];
+        }
+        sum = add_rows(sum);
+        const float mean = sum * (1.0f / D);
+#pragma unroll
+        for (int e = 0; e < 8 * NQ; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
+        const float th = limit_of(add_rows(var));
+#pragma unroll
+        for (int e = 0; e < 8 * NQ; ++e) {
+            x[e] = fminf(fmaxf(x[e], -th), th);
+            am = fmaxf(am, fabsf(x[e]));
+        }
+        int ex = 0;
+        if constexpr (SPLIT) ex = qnorm_shift(max_rows(am));
+        fac[ct] = sum != sum ? sum : p.scale * pow2i(-ex);  // (a row with NaN gives NaN: the clips would hide it)
+        const float up = pow2i(ex);
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // int4: halves 2m, 2m + 1 are nibbles m, m + 4
+                const float y = x[8 * k + (F16 ? e : e / 2 + 4 * (e % 2))] * up;
+                const _Float16 y16 = (_Float16)y;
+                qh[ct][k][e] = y16;
+                if constexpr (SPLIT) ql[ct][k][e] = (_Float16)(y - (float)y16);
+            }
+        }
+    }
+
+    f4_t acc[CT][NDT], total[CT];  // total: sum of the weights, as a row of ones would have it
+    float limit[CT], mf[CT], clip[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        limit[ct] = -INFINITY;
+        clip[ct] = p.logit_clip / fac[ct];
+        mf[ct] = -1e30f;
+        total[ct] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NDT; ++j) acc[ct][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // LDS offsets of this lane's operands in a stage
+    const int kread = (n / TI) * 1024 + ((TI == 4 ? (g ^ (n / TI)) * TI : 16 * (g >> 1) + ((g & 1) ^ (n / TI)) * TI) + n % TI) * 16;
+    constexpr int kreadstep = TI == 4 ? 256 : 512;
+
+    auto compute = [&](const int step, const int slot, const int mark, const int valid0, const int valid1) {
+        const uint8_t* st = stage + slot * kStageB;
+        f4_t sc[CT][2];
+        uint32_t fl[2], kb = 0, vb = 0;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            fl[a] = mark_word(mark, 0, a);
+            if constexpr (!F16) kb |= mark_word(mark, 1, a), vb |= mark_word(mark, 2, a);
+        }
+        // a tile that holds nodes or fewer than 16 tokens
+        const bool masked = step >= tp.prefix_steps || valid0 + valid1 < 2 * kTile;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            h8_t kh[NQ], kl[VLO ? NQ : 1];
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                kh[i] = *reinterpret_cast<const h8_t*>(st + a * kTileB + kread + i * kreadstep);
+                if constexpr (VLO) kl[i] = *reinterpret_cast<const h8_t*>(low + a * kTileB + kread + i * kreadstep);
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                f4_t c = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[i], ql[ct][i], c, 0, 0, 0);
+                }
+                if constexpr (VLO) {
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[i], qh[ct][i], c, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[i], qh[ct][i], c, 0, 0, 0);
+                sc[ct][a] = c;
+            }
+            if constexpr (CT > 1 && SPLIT) __builtin_amdgcn_sched_barrier(0);  // (registers: one tile's operands at a time)
+        }
+        if constexpr (SPLIT && F16) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                if (fl[a] == 0) continue;
+                const bool has = (fl[a] >> mark_bit(n)) & 1u;
+                const h8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    h8_t kl = *reinterpret_cast<const h8_t*>(low + mark * 2 * kTileB + a * kTileB + kread + i * kreadstep);
+                    kl = has ? kl : zero;
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) sc[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][i], sc[ct][a], 0, 0, 0);
+                }
+            }
+        }
+        settle();
+
+        // ---- softmax of column n over the lane's tokens ----
+        // bits of the lane's tokens 4g .. 4g + 3 of tile a that column ct sees
+        auto sees = [&](const int ct, const int a) -> uint32_t {
+            const int j0 = (first_tile(step) + a) * kTile + 4 * g - sp.start;  // the node that the lane's first token is
+            const uint64_t mine = bits_sh[node[ct]];
+            uint32_t seen = j0 <= -4 ? 15u
+                            : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
+                            : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
+            const int held = (a ? valid1 : valid0) - 4 * g;
+            return seen & (held >= 4 ? 15u : held > 0 ? (1u << held) - 1u : 0u);
+        };
+        if (masked || (fl[0] | fl[1] | kb) != 0) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint32_t seen = sees(ct, a);
+                    uint32_t kbw = 0;
+                    if constexpr (!F16) kbw = mark_word(mark, 1, a);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = sc[ct][a][r];
+                        if constexpr (!F16) x *= (kbw >> mark_bit(4 * g + r)) & 1u ? 16.f : 1.f;
+                        // (a key with NaN is always marked; the median would hide it)
+                        x = x != x ? x : __builtin_amdgcn_fmed3f(x, -clip[ct], clip[ct]);
+                        sc[ct][a][r] = (seen >> r) & 1u ? x : -INFINITY;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[ct][a][r] = __builtin_amdgcn_fmed3f(sc[ct][a][r], -clip[ct], clip[ct]);
+                }
+            }
+        }
+        float top[CT];
+        bool grown = false;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            top[ct] = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) top[ct] = fmaxf(top[ct], fmaxf(fmaxf(sc[ct][a][0], sc[ct][a][1]), fmaxf(sc[ct][a][2], sc[ct][a][3])));
+            grown = grown || top[ct] > limit[ct];
+        }
+        if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const float mt = max_rows(top[ct]);
+                const bool need = mt > limit[ct];
+                const float nf = fmaf(mt, fac[ct], -kHeadroom);
+                const float f = need ? __builtin_amdgcn_exp2f(mf[ct] - nf) : 1.0f;
+                limit[ct] = need ? mt + kThreshold / fac[ct] : limit[ct];
+                mf[ct] = need ? nf : mf[ct];
+                total[ct] *= f;
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) acc[ct][j] *= f;
+            }
+        }
+        h8_t ph[CT], pl[SPLIT ? CT : 1];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[ct][e / 4][e % 4], fac[ct], -mf[ct]));
+                const _Float16 w16 = (_Float16)w;
+                ph[ct][e] = w16;
+                if constexpr (SPLIT) pl[ct][e] = (_Float16)(w - (float)w16);
+            }
+            const _Float16 o = (_Float16)1.f;
+            const h8_t ones = {o, o, o, o, o, o, o, o};
+            total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[ct], total[ct], 0, 0, 0);
+            if constexpr (SPLIT) total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[ct], total[ct], 0, 0, 0);
+        }
+        if constexpr (!F16) {
+            if (vb != 0) {
+                const uint32_t vbw[2] = {mark_word(mark, 2, 0), mark_word(mark, 2, 1)};
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const _Float16 up = (vbw[e / 4] >> mark_bit(4 * g + e % 4)) & 1u ? (_Float16)16.f : (_Float16)1.f;
+                        ph[ct][e] *= up;
+                        if constexpr (SPLIT) pl[ct][e] *= up;
+                    }
+                }
+            }
+        }
+
+        // ---- O^T += V^T P^T ----
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            h8_t v[2], vl[VLO ? 2 : 1];  // of tile a: 4 tokens of d-tile 2i and of 2i + 1
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                v[a] = *reinterpret_cast<const h8_t*>(st + (2 + a) * kTileB + i * 1024 + lane * 16);
+                if constexpr (VLO) vl[a] = *reinterpret_cast<const h8_t*>(low + (2 + a) * kTileB + i * 1024 + lane * 16);
+            }
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const h8_t w = o ? __builtin_shufflevector(v[0], v[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 8, 9, 10, 11);
+                h8_t wl;
+                if constexpr (VLO) wl = o ? __builtin_shufflevector(vl[0], vl[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(vl[0], vl[1], 0, 1, 2, 3, 8, 9, 10, 11);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    f4_t& c = acc[ct][2 * i + o];
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, ph[ct], c, 0, 0, 0);
+                    if constexpr (SPLIT) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, pl[ct], c, 0, 0, 0);
+                    if constexpr (VLO) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, ph[ct], c, 0, 0, 0);
+                }
+            }
+            if constexpr (CT > 1 && SPLIT) __builtin_amdgcn_sched_barrier(0);
+        }
+        settle();
+        if (masked && (mark_word(mark, 3, 0) | mark_word(mark, 3, 1)) != 0) {
+            // rare: what is not finite reaches the rows that see it.  +inf where a visible value is +inf or NaN, and
+            // -inf where one is -inf or NaN (both: NaN), counted by products of ones; values from memory
+            const Entries e = fetch(step);
+            // (lane numbers that the compiler does not know to be loop invariants: it would keep this branch's
+            // addresses in registers all along)
+            int nn = n, gg = g;
+            asm volatile("" : "+v"(nn), "+v"(gg));
+            kernel_args* late = late_args();
+#pragma unroll 1
+            for (int a = 0; a < 2; ++a) {
+                const Where w0 = where(step, 0, e), w1 = where(step, 1, e);
+                const Where w = {a ? w1.bh : w0.bh, a ? w1.slot0 : w0.slot0, a ? w1.valid : w0.valid};
+                uint32_t seen[CT];
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) seen[ct] = sees(ct, a);
+#pragma unroll
+                for (int j = 0; j < NDT; ++j) {
+                    const uint32_t d = F16 ? 32 * (j / 2) + 2 * nn + j % 2 : 16 * j + nn;
+                    h4_t plus, minus;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = 4 * gg + r < w.valid;
+                        const float v = in ? tree_value<DT, D>(late->v, late->vs, (uint32_t)P, w.bh, (uint32_t)(w.slot0 + 4 * gg + r), d) : 0.f;
+                        plus[r] = in && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                        minus[r] = in && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                    }
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        h4_t vis;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) vis[r] = (seen[ct] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
+                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                        const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
+                        const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
+                        settle();
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
+                            acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    // Step s's loads are in slot (s - lo) % (AHEAD + 1); those of its wave have landed once no more than
+    // the loads of the AHEAD - 1 steps after it are on their way.
+    wait_loads<(AHEAD - 1) * kLoads>();
+    prepare(lo, (held[0] >> (8 * my_tile)) & 0xff, 0, 0, 0);
+    barrier_lds();
+    int slot = 0, mark = 0;
+    for (int step = lo; step < hi; ++step) {
+        const int next = slot == AHEAD ? 0 : slot + 1;
+        const Entries e = ahead;
+        ahead = fetch(step + AHEAD + 1);
+        held[AHEAD] = load_step(step + AHEAD, slot == 0 ? AHEAD : slot - 1, e);
+        compute(step, F16 ? slot : 0, mark, held[0] & 0xff, held[0] >> 8);
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) held[s] = held[s + 1];
+        wait_loads<(AHEAD - 1) * kLoads>();
+        if constexpr (F16) {
+            mark ^= 1;
+            prepare(step + 1, (held[0] >> (8 * my_tile)) & 0xff, next, mark, 0);
+        } else {
+            barrier_lds();  // (every wave has read this step's rows)
+            prepare(step + 1, (held[0] >> (8 * my_tile)) & 0xff, 0, 0, next);
+        }
+        barrier_lds();
+        slot = next;
+    }
+    wait_loads<0>();
+    settle();
+
+    kernel_args* late = late_args();
+    const int group = (int)late->group;
+    const bool whole = tp.count == 1;
+    const size_t state = ((size_t)b * (late->hkv * late->col_groups) + item) * late->parts + part;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int tile = wave * CT + ct;
+        const float sum = total[ct][0];
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < NDT; ++j) reinterpret_cast<f4_t*>(late->part_acc)[((state * (W * CT) + tile) * NDT + j) * 64 + lane] = acc[ct][j];
+            if (g == 0) {
+                float* ml = late->part_ml + ((state * (W * CT) + tile) * 16 + n) * 2;
+                ml[0] = mf[ct];
+                ml[1] = sum;
+            }
+            continue;
+        }
+        const int c = (ctile0 + ct) * 16 + n;
+        if (c >= cols) continue;
+        const int i = c / group;
+        IO* dst = reinterpret_cast<IO*>(late->out) + (((size_t)b * late->nodes + i) * late->hq + (size_t)h * group + (c - i * group)) * D;
+        const bool empty = i >= sp.len || sum == 0.f;
+#pragma unroll
+        for (int j = 0; j < NDT; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : acc[ct][j][r] / sum);
+        }
+    }
+}
+
+template <int DT, int D, typename IO, int CT, int W>
+void launch(const TreeParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((tree_wide<DT, D, IO, CT, W>), dim3(p.hkv * p.col_groups * p.parts, p.batch), dim3(W * 64), 0, s, p);
+    if (p.parts > 1) launch_merge<DT, D, IO>(p, W * CT, s);
+}
+
+template <int DT, int D, typename IO>
+void launch_any(const TreeParams& p, uint32_t ct, hipStream_t s) {
+    if (p.col_waves == 8) launch<DT, D, IO, 2, 8>(p, s);
+    else if (ct == 2) launch<DT, D, IO, 2, 4>(p, s);
+    else launch<DT, D, IO, 1, 4>(p, s);
+}
+
+}  // namespace
+
+#define TREE_LAUNCH_(name, dt, d)                                            \
+    void name(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s) { \
+        if (io == VSPEC_KV_F32) launch_any<dt, d, float>(p, ct, s);          \
+        else launch_any<dt, d, _Float16>(p, ct, s);                          \
+    }
+#if VSPEC_HEAD_DIM == 64
+TREE_LAUNCH_(launch_tree_wide_f16_d64, VSPEC_KV_F16, 64)
+TREE_LAUNCH_(launch_tree_wide_int4_d64, VSPEC_KV_INT4, 64)
+#else
+TREE_LAUNCH_(launch_tree_wide_f16_d128, VSPEC_KV_F16, 128)
+TREE_LAUNCH_(launch_tree_wide_int4_d128, VSPEC_KV_INT4, 128)
+#endif
+#undef TREE_LAUNCH_
+
+}  // namespace vkv

@@ -128,6 +128,7 @@ void launch_tree_wide_f16_d128(const TreeParams& p, int32_t io, uint32_t ct, hip
 void launch_tree_wide_int4_d64(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
 void launch_tree_wide_int4_d128(const TreeParams& p, int32_t io, uint32_t ct, hipStream_t s);
 // 16-token tiles of a step
+constexpr int wide_step_tiles(bool f32_rows, int ct) { return f32_rows || ct > 1 ? 2 : 4; }
 constexpr int tree_step_tiles(int dtype) { return dtype == VSPEC_KV_F32 ? 1 : 2; }
 
 }  // namespace vkv

@@ -70,10 +70,11 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     const uint64_t cap = (uint64_t)d->max_blocks_per_seq * d->kv.block_tokens;
     uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
     if (bound > cap) bound = cap;
-    const uint32_t per = 16 * tree_step_tiles(d->kv.dtype);
+    const bool f32_rows = d->io_dtype == VSPEC_KV_F32;
+    const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype));
     const uint64_t steps = (bound + per - 1) / per;
     const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups * d->batch;
-    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : pl.ct == 1 && d->io_dtype == VSPEC_KV_F16 ? 3 : 2) : 1);
+    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : 2) : 1);
     uint64_t parts = items ? slots / items : 1;
     const uint64_t most = pl.wide ? steps / 4 : steps * pl.col_waves / 8;  // two steps a wave
     if (parts > most) parts = most;

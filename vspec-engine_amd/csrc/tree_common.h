@@ -74,10 +74,9 @@ __device__ __forceinline__ void int4_values(uint32_t codes, const h2_t (&scale)[
     }
 }
 
-// The parts of one column tile of an item.
-template <int DT, int D, typename IO>
+// The parts of one column tile of an item, cut in steps of NT tiles.
+template <int DT, int D, typename IO, int NT>
 __global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t tiles) {
-    constexpr int NT = tree_step_tiles(DT);
     constexpr int NDT = D / 16;
     const uint32_t b = blockIdx.y, item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
     const uint32_t h = item / p.col_groups, cg = item - h * p.col_groups;
@@ -109,9 +108,9 @@ __global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t tiles) 
     }
 }
 
-template <int DT, int D, typename IO>
+template <int DT, int D, typename IO, int NT>
 void launch_merge(const TreeParams& p, uint32_t tiles, hipStream_t s) {
-    hipLaunchKernelGGL((tree_merge<DT, D, IO>), dim3(p.hkv * p.col_groups * tiles, p.batch), dim3(256), 0, s, p, tiles);
+    hipLaunchKernelGGL((tree_merge<DT, D, IO, NT>), dim3(p.hkv * p.col_groups * tiles, p.batch), dim3(256), 0, s, p, tiles);
 }
 
 }  // namespace

@@ -765,7 +765,7 @@ void launch(const TreeParams& p, uint32_t ct, hipStream_t s) {
         default: hipLaunchKernelGGL((tree_attention<DT, D, IO, 2>), grid, dim3(256), 0, s, p); break;
     }
     if (p.parts > 1) {
-        launch_merge<DT, D, IO>(p, p.col_waves * ct, s);
+        launch_merge<DT, D, IO, tree_step_tiles(DT)>(p, p.col_waves * ct, s);
     }
 }
 

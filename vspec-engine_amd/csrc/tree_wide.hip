@@ -30,32 +30,41 @@ __device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes)
 
 __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The chunk of its row in lane (position) l of a set of TI rows (set m of a tile), and the position's inverse:
+// the 16 rows' chunks of one operand then lie in different banks.
+template <int D>
+__device__ __forceinline__ int chunk_of(int m, int l) {
+    constexpr int CPT = D / 8;
+    const int t = l / CPT;
+    return (l % CPT) ^ (D == 128 ? 4 * m + t : 4 * m + (t >> 1));
+}
+
 template <typename IO>
 constexpr bool SPLIT_IO = sizeof(IO) == 4;
 
 template <int DT, int D, typename IO, int CT, int W>
 __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree_wide(TreeParams p) {
     constexpr bool F16 = DT == VSPEC_KV_F16;
-    constexpr bool SPLIT = sizeof(IO) == 4;   // q and p in two f16 parts
+    constexpr bool SPLIT = SPLIT_IO<IO>;      // q and p in two f16 parts
     constexpr bool VLO = SPLIT && !F16;       // K and V in two f16 parts
     constexpr int NQ = D / 32, NDT = D / 16;
+    constexpr int KT = wide_step_tiles(SPLIT, CT);  // 16-token tiles of a step
     constexpr int CPT = D / 8;                // 8-element chunks of a row
     constexpr int TI = 64 / CPT;              // rows that a wave takes at a time, a chunk a lane
-    constexpr int SETS = W == 4 && D == 128 ? 2 : 1;
-    constexpr int TPO = TI * SETS;            // rows of a step that a wave looks after: TPO w ..
-    constexpr int OWNERS = 32 / TPO;          // waves that look after rows
-    constexpr int CL = 16 / TI;
+    constexpr int TPO = 16 * KT / W < TI ? TI : 16 * KT / W;  // rows of a step that a wave looks after: TPO w .., of one tile
+    constexpr int SETS = TPO / TI;
+    constexpr int OWNERS = 16 * KT / TPO;     // waves that look after rows
     constexpr int kTileB = 32 * D;            // bytes of a tile in f16
-    constexpr int kStageB = 4 * kTileB;       // K of both tiles, V of both
-    constexpr int DEPTH = F16 ? (W == 8 ? 4 : 3) : 1;
-    constexpr int RAW = 4;                    // steps of codes in the ring
+    constexpr int kStageB = 2 * KT * kTileB;  // K of all tiles, V of all
+    constexpr int DEPTH = F16 ? (KT == 4 ? 2 : W == 8 ? 4 : 3) : 1;
+    constexpr int RAW = 3;                    // steps of codes in the ring
     constexpr int kRawB = F16 ? 16 : 512 * SETS + 512;  // of a wave and step: K, V, K scales, V scales
     __shared__ __align__(16) uint8_t stage[DEPTH * kStageB];
-    __shared__ __align__(16) uint8_t low[SPLIT ? (F16 ? 2 * 2 * kTileB : kStageB) : 16];  // low parts: f16 [slot][K], int4 as a stage
+    __shared__ __align__(16) uint8_t low[SPLIT ? (F16 ? 2 * KT * kTileB : kStageB) : 16];  // low parts: f16 [mark][K], int4 as a stage
     __shared__ __align__(16) uint8_t raw[F16 ? 16 : RAW * OWNERS * kRawB];
-    // a bit for each row of a step, TPO to the byte of its wave: clipped or not finite; K (int4) and V (int4)
-    // hold a 16th of the value; V held something that is not finite
-    __shared__ __align__(8) uint8_t marks[2][4][8];
+    // a bit for each row of a step, whole bytes of each wave's: clipped or not finite; K (int4) and V (int4) hold a 16th of the
+    // value; V held something that is not finite
+    __shared__ __align__(8) uint16_t marks[2][4][4];
     __shared__ uint64_t bits_sh[64];
 
     const int lane = threadIdx.x & 63;
@@ -65,7 +74,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     const uint32_t item = (uint32_t)uniform((int)(blockIdx.x / p.parts)), part = blockIdx.x - item * p.parts;
     const uint32_t h = (uint32_t)uniform((int)(item / p.col_groups)), cg = item - h * p.col_groups;
     const TreeSpan sp = tree_span(p, b);
-    const TreeParts tp = tree_parts<2>(p, sp);
+    const TreeParts tp = tree_parts<KT>(p, sp);
     if ((int)part >= tp.count) return;
     const int lo = (int)part * tp.chunk, hi = min(lo + tp.chunk, tp.steps);
     if (threadIdx.x < 64) bits_sh[threadIdx.x] = threadIdx.x < p.nodes ? tree_bits(p, b, threadIdx.x, sp.len) : 0;
@@ -81,56 +90,49 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     const uint32_t magic = own_scalar(p.block_magic), shift = own_scalar(p.block_shift);
     const float alpha = own_scalar(p.alpha), input_clip = own_scalar(p.input_clip);
 
-    // Steps ahead of the one at work: their table entries are read a step before their loads go out, and how
-    // many tokens their tiles hold stays in scalar registers until they are worked on.
-    struct Entries {
-        int block[2], used[2];
+    // The tiles of the next 64 / KT steps, a lane each: where a tile lies (token index in the pool), its slot in the
+    // block and how many tokens it holds (0: it is not read).  Read lane by lane, this costs a step two scalar
+    // moves a tile; table look-ups of each step were 170 instructions.
+    constexpr int kSpan = 64 / KT;
+    size_t t_token = 0;
+    int t_info = 0;  // slot0 << 5 | tokens
+    auto look_up = [&](const int first) {
+        const int step = first + lane / KT, a = lane % KT;
+        const int tile = step < tp.prefix_steps ? KT * step + a : tp.prefix_tiles + KT * (step - tp.prefix_steps) + a;
+        const bool in = step < hi && tile < (step < tp.prefix_steps ? tp.prefix_tiles : tp.tiles);
+        const int row = in ? tree_block_of(magic, shift, tile) : 0;
+        const int entry = tables[row];
+        const int room = used ? used[row] : P;
+        const bool ok = in && entry >= 0 && (uint32_t)entry < num_blocks;
+        const int slot0 = ok ? tile * kTile - row * P : 0;
+        t_token = ((size_t)(ok ? entry : 0) * hkv + h) * P + slot0;
+        t_info = slot0 << 5 | (ok ? min(min(kTile, sp.end - tile * kTile), max(0, room - slot0)) : 0);
     };
-    auto first_tile = [&](const int step) { return step < tp.prefix_steps ? 2 * step : tp.prefix_tiles + 2 * (step - tp.prefix_steps); };
-    auto last_tile = [&](const int step) { return step < tp.prefix_steps ? tp.prefix_tiles : tp.tiles; };
-    auto fetch = [&](int step) -> Entries {
-        step = __builtin_amdgcn_readfirstlane(step);
-        Entries e;
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const int tile = first_tile(step) + a;
-            const bool in = step < hi && tile < last_tile(step);
-            const int row = in ? tree_block_of(magic, shift, tile) : 0;
-            const int entry = as_const(tables)[row];
-            e.block[a] = in && entry >= 0 && (uint32_t)entry < num_blocks ? entry : -1;
-            e.used[a] = used ? as_const(used)[row] : P;
-        }
-        return e;
-    };
-    // where tile a of a step lies, and how many tokens it holds (0: it is not read)
     struct Where {
-        size_t bh;
+        size_t token;
         int slot0, valid;
     };
-    auto where = [&](const int step, const int a, const Entries& e) -> Where {
-        const int tile = first_tile(step) + a;
-        const bool ok = e.block[a] >= 0;
-        Where w;
-        w.bh = (size_t)(ok ? e.block[a] : 0) * hkv + h;
-        w.slot0 = ok ? tile * kTile - tree_block_of(magic, shift, tile) * P : 0;
-        w.valid = ok ? min(min(kTile, sp.end - tile * kTile), max(0, e.used[a] - w.slot0)) : 0;
-        return w;
+    int table0 = lo;  // the first step of the table
+    auto where = [&](const int step, const int a) -> Where {
+        const int l = uniform((step - table0) * KT + a);
+        const uint32_t t0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)t_token, l);
+        const uint32_t t1 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(t_token >> 32), l);
+        const int info = __builtin_amdgcn_readlane(t_info, l);
+        return {(size_t)t1 << 32 | t0, info >> 5, info & 31};
     };
+    auto first_tile = [&](const int step) { return step < tp.prefix_steps ? KT * step : tp.prefix_tiles + KT * (step - tp.prefix_steps); };
 
     // ---- loads of this wave's share of a step ----
-    const bool owner = wave < OWNERS;
-    const int my_tile = (TPO * wave) / kTile & 1;    // the tile of its rows
-    const int my_part = (TPO * wave) % kTile / TPO;  // and which TPO rows of it
+    const bool owner = OWNERS == W || wave < OWNERS;
+    const int my_tile = owner ? TPO * wave / kTile : 0;  // the tile of its rows
+    const int my_part = TPO * wave % kTile / TPO;    // and which TPO rows of it
     uint32_t koff[SETS], voff[SETS];                 // f16: byte offsets of this lane's chunks in the tile
     if constexpr (F16) {
 #pragma unroll
         for (int k = 0; k < SETS; ++k) {
-            // rows TI m .. of the tile.  Lane (position) l of the 1 KB holds chunk c of row t such that the 16 rows
-            // of one chunk lie in different banks
-            const int m = my_part * SETS + k, t = lane % TI;
-            const int c = CL * (lane / 16) + (((lane % 16) / TI) ^ m);
-            koff[k] = (uint32_t)((TI * m + t) * 2 * D + 16 * c);
-            voff[k] = (uint32_t)(g * 8 * D + (32 * m + 2 * n) * 8);  // V operands m of the tile
+            const int m = my_part * SETS + k;  // rows TI m .. of the tile, V operands m
+            koff[k] = (uint32_t)((TI * m + lane / CPT) * 2 * D + 16 * chunk_of<D>(m, lane));
+            voff[k] = (uint32_t)(g * 8 * D + (32 * m + 2 * n) * 8);
         }
     }
     const uint32_t stage0 = lds_addr(stage), raw0 = lds_addr(raw);
@@ -138,19 +140,19 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
         if (!owner) return;
         if constexpr (F16) {
             const uint32_t bytes = w.valid > 0 ? kTileB : 0;
-            const size_t at = (w.bh * P + w.slot0) * (size_t)(2 * D);
+            const size_t at = w.token * (size_t)(2 * D);
             const rsrc_t kr = uniform_rsrc(kdata + at, bytes), vr = uniform_rsrc(vdata + at, bytes);
             const uint32_t dst = stage0 + slot * kStageB + my_tile * kTileB + my_part * SETS * 1024;
 #pragma unroll
             for (int k = 0; k < SETS; ++k) lds_load16(__builtin_amdgcn_readfirstlane(dst + 1024 * k), kr, koff[k]);
 #pragma unroll
-            for (int k = 0; k < SETS; ++k) lds_load16(__builtin_amdgcn_readfirstlane(dst + 2 * kTileB + 1024 * k), vr, voff[k]);
+            for (int k = 0; k < SETS; ++k) lds_load16(__builtin_amdgcn_readfirstlane(dst + KT * kTileB + 1024 * k), vr, voff[k]);
         } else {
             const uint32_t bytes = w.valid > 0 ? 8 * D : 0;
-            const size_t at = (w.bh * P + w.slot0) * (size_t)(D / 2);
+            const size_t at = w.token * (size_t)(D / 2);
             const rsrc_t kr = uniform_rsrc(kdata + at, bytes), vr = uniform_rsrc(vdata + at, bytes);
-            const rsrc_t ksr = uniform_rsrc(kscales + w.bh * NQ * P + w.slot0, w.valid > 0 ? (uint32_t)((NQ - 1) * P * 2 + 32) : 0u);
-            const rsrc_t vsr = uniform_rsrc(vscales + (w.bh * P + w.slot0) * NQ, w.valid > 0 ? 32 * NQ : 0);
+            const rsrc_t ksr = uniform_rsrc(kscales + (w.token - w.slot0) * NQ + w.slot0, w.valid > 0 ? (uint32_t)((NQ - 1) * P * 2 + 32) : 0u);
+            const rsrc_t vsr = uniform_rsrc(vscales + w.token * NQ, w.valid > 0 ? 32 * NQ : 0);
             const uint32_t dst = raw0 + (slot * OWNERS + wave) * kRawB;
             const uint32_t from = my_part * TPO * (D / 2) + 4 * lane;
 #pragma unroll
@@ -165,35 +167,19 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     constexpr int kLoads = F16 ? 2 * SETS : 2 * SETS + 2;  // of a step
 
     // ---- what a wave does to its rows of a step before all waves read them ----
-    // sum over the lanes that hold a row: f16 lanes with the same lane % TI, int4 CPT adjacent ones
-    auto row_sum = [&](float x) {
-        if constexpr (F16) {
-            x += row_dpp<kRowRor8>(x);
-            if constexpr (TI == 4) x += row_dpp<kRowRor4>(x);
-            return add_rows(x);
-        } else {
-            return group_sum<CPT>(x);
-        }
-    };
+    // (a row's chunks lie in CPT adjacent lanes)
+    auto row_sum = [&](float x) { return group_sum<CPT>(x); };
     // the bits of its rows (of set k) from a ballot in which any lane of a row speaks for it
     auto row_bits = [&](uint64_t m) -> uint32_t {
-        if constexpr (F16) {
-            m |= m >> 32;
-            m |= m >> 16;
-            m |= m >> 8;
-            if constexpr (TI == 4) m |= m >> 4;
-            return (uint32_t)m & ((1u << TI) - 1u);
-        } else {
-            uint32_t r = 0;
+        uint32_t r = 0;
 #pragma unroll
-            for (int t = 0; t < TI; ++t) r |= (uint32_t)((m >> (CPT * t)) & ((1ull << CPT) - 1)) ? 1u << t : 0u;
-            return r;
-        }
+        for (int t = 0; t < TI; ++t) r |= (uint32_t)((m >> (CPT * t)) & ((1ull << CPT) - 1)) ? 1u << t : 0u;
+        return r;
     };
     auto limit_of = [&](float var) { return fminf(fmaxf(1e-6f, alpha * sqrtf(var * (1.0f / D))), input_clip); };
     auto prepare = [&](const int step, const int valid, const int slot, const int mark, const int raw_slot) {
         if (!owner) return;
-        uint32_t clipped = 0, kbig = 0, vbig = 0, wild = 0;
+        uint32_t clipped = 0, kbig = 0, vbig = 0, odd_v = 0;
         // V of slots without a token may hold any bits and becomes zeros.  In tiles that hold nodes so does
         // what is not finite: in the products 0 * inf would reach the rows that do not see it
         const bool tree = (first_tile(step) + my_tile) * kTile + valid > sp.start;
@@ -219,7 +205,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                 const float th1 = fminf(fmaxf(1e-6f, alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), input_clip);
                 // the margins of the decode's screen; !(<=) also takes what is not finite
                 const bool flag = !(mx <= th1 * (1.0f - 0.0009765625f)) || var1 <= ex2 * 0.0009765625f;
-                const int row = TI * (my_part * SETS + k) + lane % TI;
+                const int row = TI * (my_part * SETS + k) + lane / CPT;
                 const uint64_t any = __builtin_amdgcn_ballot_w64(flag && row < valid);
                 if (any == 0) continue;
                 // exactly, for the rows that it takes: two-pass deviation, the clipped row in two f16 parts.
@@ -244,15 +230,15 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                     yh[e] = (_Float16)y;
                     yl[e] = (_Float16)(y - (float)yh[e]);
                 }
-                if ((rows >> (lane % TI)) & 1u) {
+                if ((rows >> (lane / CPT)) & 1u) {
                     *reinterpret_cast<h8_t*>(mine + 1024 * k) = yh;
-                    if constexpr (SPLIT) *reinterpret_cast<h8_t*>(low + mark * 2 * kTileB + my_tile * kTileB + (my_part * SETS + k) * 1024 + 16 * lane) = yl;
+                    if constexpr (SPLIT) *reinterpret_cast<h8_t*>(low + mark * KT * kTileB + my_tile * kTileB + (my_part * SETS + k) * 1024 + 16 * lane) = yl;
                 }
             }
             if (tree || valid < kTile) {
 #pragma unroll
                 for (int k = 0; k < SETS; ++k) {
-                    h8_t* at = reinterpret_cast<h8_t*>(mine + 2 * kTileB + 1024 * k);
+                    h8_t* at = reinterpret_cast<h8_t*>(mine + KT * kTileB + 1024 * k);
                     h8_t v = *at;
                     bool out = false;
 #pragma unroll
@@ -263,7 +249,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                         v[e] = held && !odd ? v[e] : (_Float16)0.f;
                     }
                     *at = v;
-                    wild |= __builtin_amdgcn_ballot_w64(out) != 0 ? 1u : 0u;
+                    odd_v |= __builtin_amdgcn_ballot_w64(out) != 0 ? 1u : 0u;
                 }
             }
         } else {
@@ -324,7 +310,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                     }
                 }
                 const int m = row / TI, t = row % TI;
-                const int at = my_tile * kTileB + m * 1024 + (16 * (c / CL) + ((c % CL) ^ m) * TI + t) * 16;
+                const int at = my_tile * kTileB + m * 1024 + (CPT * t + chunk_of<D>(m, CPT * t + c)) * 16;
                 *reinterpret_cast<h8_t*>(stage + at) = yh;
                 if constexpr (VLO) *reinterpret_cast<h8_t*>(low + at) = yl;
             }
@@ -344,7 +330,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                     sw[e] = a | (z << 16);
                 }
                 if (tree && __builtin_amdgcn_ballot_w64(top >= 0x7C00u) != 0) {
-                    wild = 1;
+                    odd_v = 1;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         sw[e] &= ((sw[e] & 0x7fffu) < 0x7C00u ? 0xffffu : 0u) | (((sw[e] >> 16) & 0x7fffu) < 0x7C00u ? 0xffff0000u : 0u);
@@ -361,48 +347,59 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                         const bool is = most >= kBigScale;
                         sp2[r / 2][r % 2] *= is ? (_Float16)0.0625f : (_Float16)1.f;
                         const uint64_t all = __builtin_amdgcn_ballot_w64(is);
-                        // the wave's V words belong to TPO tokens, 4 for each row group in it
+                        // the words of a set belong to 4 tokens (64-element rows: 8, 4 in each half of the wave)
                         if constexpr (NQ == 4) vbig |= all ? 1u << (4 * k + r) : 0u;
-                        else vbig |= ((uint32_t)all ? 1u << r : 0u) | ((uint32_t)(all >> 32) ? 16u << r : 0u);
+                        else vbig |= ((uint32_t)all ? 1u << (8 * k + r) : 0u) | ((uint32_t)(all >> 32) ? 16u << (8 * k + r) : 0u);
                     }
                 }
                 h4_t ve, vo, vel, vol;
                 int4_values<VLO>(w, sp2, ve, vo, vel, vol);
-                const int at = 2 * kTileB + my_tile * kTileB + c * 1024 + (chunk % 64) * 16;
+                const int at = KT * kTileB + my_tile * kTileB + c * 1024 + (chunk % 64) * 16;
                 *reinterpret_cast<h8_t*>(stage + at) = join(ve, vo);
                 if constexpr (VLO) *reinterpret_cast<h8_t*>(low + at) = join(vel, vol);
             }
         }
         if (lane == 0) {
-            marks[mark][0][wave] = (uint8_t)clipped;
-            marks[mark][1][wave] = (uint8_t)kbig;
-            marks[mark][2][wave] = (uint8_t)vbig;
-            marks[mark][3][wave] = (uint8_t)wild;
+            const uint32_t m[4] = {clipped, kbig, vbig, odd_v};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (TPO == 16) marks[mark][i][wave] = (uint16_t)m[i];
+                else reinterpret_cast<uint8_t*>(marks[mark][i])[wave] = (uint8_t)m[i];
+            }
         }
     };
-    // the marks of tile a: bit mark_bit(n) of the word speaks for its token n
-    auto mark_word = [&](const int mark, const int which, const int a) -> uint32_t {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(&marks[mark][which][TPO == 4 ? 4 * a : 0]);
-        return __builtin_amdgcn_readfirstlane(TPO == 4 ? w : (w >> (16 * a)) & 0xffffu);
+    // the marks of a step, and of its tile a alone: 16 bits
+    auto marks_of = [&](const int mark, const int which) -> uint64_t {
+        const uint2 w = *reinterpret_cast<const uint2*>(marks[mark][which]);
+        const uint64_t all = (uint64_t)(uint32_t)uniform((int)w.y) << 32 | (uint32_t)uniform((int)w.x);
+        return KT == 4 || TPO == 4 ? all : all & 0xffffffffull;
     };
-    auto mark_bit = [](int t) { return TPO == 4 ? 8 * (t >> 2) + (t & 3) : t; };
+    auto tile_marks = [](uint64_t m, int a) -> uint32_t {
+        if constexpr (TPO == 4) {
+            const uint32_t w = (uint32_t)(m >> (32 * a));  // 4 bits in each byte
+            return (w & 0xfu) | (w >> 4 & 0xf0u) | (w >> 8 & 0xf00u) | (w >> 12 & 0xf000u);
+        } else {
+            return (uint32_t)(m >> (16 * a)) & 0xffffu;
+        }
+    };
 
     // ---- the first steps on their way, then q ----
     constexpr int AHEAD = F16 ? DEPTH - 1 : RAW - 1;
-    int held[AHEAD + 1];  // tokens of the tiles (second: 256 times) of the step at work and of those on their way
-    auto load_step = [&](int step, const int slot, const Entries& e) -> int {
-        step = __builtin_amdgcn_readfirstlane(step);
-        const Where w0 = where(step, 0, e), w1 = where(step, 1, e);
-        load({my_tile ? w1.bh : w0.bh, my_tile ? w1.slot0 : w0.slot0, my_tile ? w1.valid : w0.valid}, slot);
-        return w0.valid | (w1.valid << 8);
-    };
-    Entries ahead = fetch(lo);
+    int held[AHEAD + 1];  // tokens of the tiles of the step at work and of those on their way, 5 bits each
+    look_up(lo);
+    auto load_step = [&](const int step, const int slot) -> int {
+        if (step == table0 + kSpan) {
+            table0 = step;
+            look_up(step);
+        }
+        int tokens = 0;
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {
-        const Entries e = ahead;
-        ahead = fetch(lo + s + 1);
-        held[s] = load_step(lo + s, s, e);
-    }
+        for (int a = 0; a < KT; ++a) tokens |= (uniform(__builtin_amdgcn_readlane(t_info, (step - table0) * KT + a)) & 31) << (5 * a);
+        load(where(step, my_tile), slot);
+        return tokens;
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) held[s] = load_step(lo + s, s);
 
     const int cols = (int)(p.nodes * p.group);
     const int ctile0 = ((int)cg * W + wave) * CT;
@@ -473,28 +470,36 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
         for (int j = 0; j < NDT; ++j) acc[ct][j] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // LDS offsets of this lane's operands in a stage
-    const int kread = (n / TI) * 1024 + ((TI == 4 ? (g ^ (n / TI)) * TI : 16 * (g >> 1) + ((g & 1) ^ (n / TI)) * TI) + n % TI) * 16;
-    constexpr int kreadstep = TI == 4 ? 256 : 512;
+    // LDS offset of this lane's K operand 0 in a tile; operand i is at kread ^ 64 i
+    const int kread = (n / TI) * 1024 + (CPT * (n % TI) + chunk_of<D>(n / TI, CPT * (n % TI) + g)) * 16;
 
-    auto compute = [&](const int step, const int slot, const int mark, const int valid0, const int valid1) {
+    // bits of the lane's tokens 4g .. 4g + 3 of a tile that column ct sees
+    auto sees = [&](const int ct, const int tile, const int valid) -> uint32_t {
+        const int j0 = tile * kTile + 4 * g - sp.start;  // the node that the lane's first token is
+        const uint64_t mine = bits_sh[node[ct]];
+        const uint32_t seen = j0 <= -4 ? 15u
+                              : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
+                              : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
+        const int left = valid - 4 * g;
+        return seen & (left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u);
+    };
+    bool wild = false;  // some step's V held what is not finite, among nodes
+
+    auto compute = [&](const int step, const int slot, const int mark, const int tokens) {
         const uint8_t* st = stage + slot * kStageB;
-        f4_t sc[CT][2];
-        uint32_t fl[2], kb = 0, vb = 0;
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            fl[a] = mark_word(mark, 0, a);
-            if constexpr (!F16) kb |= mark_word(mark, 1, a), vb |= mark_word(mark, 2, a);
-        }
+        f4_t sc[CT][KT];
+        const uint64_t fl = marks_of(mark, 0);
+        uint64_t kb = 0, vb = 0;
+        if constexpr (!F16) kb = marks_of(mark, 1), vb = marks_of(mark, 2);
         // a tile that holds nodes or fewer than 16 tokens
-        const bool masked = step >= tp.prefix_steps || valid0 + valid1 < 2 * kTile;
+        const bool masked = step >= tp.prefix_steps || tokens != (KT == 4 ? 0x84210 : 0x210);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < KT; ++a) {
             h8_t kh[NQ], kl[VLO ? NQ : 1];
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
-                kh[i] = *reinterpret_cast<const h8_t*>(st + a * kTileB + kread + i * kreadstep);
-                if constexpr (VLO) kl[i] = *reinterpret_cast<const h8_t*>(low + a * kTileB + kread + i * kreadstep);
+                kh[i] = *reinterpret_cast<const h8_t*>(st + a * kTileB + (kread ^ (64 * i)));
+                if constexpr (VLO) kl[i] = *reinterpret_cast<const h8_t*>(low + a * kTileB + (kread ^ (64 * i)));
             }
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
@@ -514,45 +519,35 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
             if constexpr (CT > 1 && SPLIT) __builtin_amdgcn_sched_barrier(0);  // (registers: one tile's operands at a time)
         }
         if constexpr (SPLIT && F16) {
+            if (fl != 0) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                if (fl[a] == 0) continue;
-                const bool has = (fl[a] >> mark_bit(n)) & 1u;
-                const h8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (int a = 0; a < KT; ++a) {
+                    if (tile_marks(fl, a) == 0) continue;
+                    const bool has = (tile_marks(fl, a) >> n) & 1u;
+                    const h8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    h8_t kl = *reinterpret_cast<const h8_t*>(low + mark * 2 * kTileB + a * kTileB + kread + i * kreadstep);
-                    kl = has ? kl : zero;
+                    for (int i = 0; i < NQ; ++i) {
+                        h8_t kl = *reinterpret_cast<const h8_t*>(low + (mark * KT + a) * kTileB + (kread ^ (64 * i)));
+                        kl = has ? kl : zero;
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) sc[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][i], sc[ct][a], 0, 0, 0);
+                        for (int ct = 0; ct < CT; ++ct) sc[ct][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[ct][i], sc[ct][a], 0, 0, 0);
+                    }
                 }
             }
         }
         settle();
 
         // ---- softmax of column n over the lane's tokens ----
-        // bits of the lane's tokens 4g .. 4g + 3 of tile a that column ct sees
-        auto sees = [&](const int ct, const int a) -> uint32_t {
-            const int j0 = (first_tile(step) + a) * kTile + 4 * g - sp.start;  // the node that the lane's first token is
-            const uint64_t mine = bits_sh[node[ct]];
-            uint32_t seen = j0 <= -4 ? 15u
-                            : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
-                            : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
-            const int held = (a ? valid1 : valid0) - 4 * g;
-            return seen & (held >= 4 ? 15u : held > 0 ? (1u << held) - 1u : 0u);
-        };
-        if (masked || (fl[0] | fl[1] | kb) != 0) {
+        if (masked || (fl | kb) != 0) {
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const uint32_t seen = sees(ct, a);
-                    uint32_t kbw = 0;
-                    if constexpr (!F16) kbw = mark_word(mark, 1, a);
+                for (int a = 0; a < KT; ++a) {
+                    const uint32_t seen = sees(ct, first_tile(step) + a, (tokens >> (5 * a)) & 31);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float x = sc[ct][a][r];
-                        if constexpr (!F16) x *= (kbw >> mark_bit(4 * g + r)) & 1u ? 16.f : 1.f;
+                        if constexpr (!F16) x *= (tile_marks(kb, a) >> (4 * g + r)) & 1u ? 16.f : 1.f;
                         // (a key with NaN is always marked; the median would hide it)
                         x = x != x ? x : __builtin_amdgcn_fmed3f(x, -clip[ct], clip[ct]);
                         sc[ct][a][r] = (seen >> r) & 1u ? x : -INFINITY;
@@ -563,7 +558,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
+                for (int a = 0; a < KT; ++a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sc[ct][a][r] = __builtin_amdgcn_fmed3f(sc[ct][a][r], -clip[ct], clip[ct]);
                 }
@@ -575,7 +570,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
         for (int ct = 0; ct < CT; ++ct) {
             top[ct] = -INFINITY;
 #pragma unroll
-            for (int a = 0; a < 2; ++a) top[ct] = fmaxf(top[ct], fmaxf(fmaxf(sc[ct][a][0], sc[ct][a][1]), fmaxf(sc[ct][a][2], sc[ct][a][3])));
+            for (int a = 0; a < KT; ++a) top[ct] = fmaxf(top[ct], fmaxf(fmaxf(sc[ct][a][0], sc[ct][a][1]), fmaxf(sc[ct][a][2], sc[ct][a][3])));
             grown = grown || top[ct] > limit[ct];
         }
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
@@ -592,31 +587,36 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                 for (int j = 0; j < NDT; ++j) acc[ct][j] *= f;
             }
         }
-        h8_t ph[CT], pl[SPLIT ? CT : 1];
+        h8_t ph[CT][KT / 2], pl[SPLIT ? CT : 1][KT / 2];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[ct][e / 4][e % 4], fac[ct], -mf[ct]));
-                const _Float16 w16 = (_Float16)w;
-                ph[ct][e] = w16;
-                if constexpr (SPLIT) pl[ct][e] = (_Float16)(w - (float)w16);
+            for (int u = 0; u < KT / 2; ++u) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[ct][2 * u + e / 4][e % 4], fac[ct], -mf[ct]));
+                    const _Float16 w16 = (_Float16)w;
+                    ph[ct][u][e] = w16;
+                    if constexpr (SPLIT) pl[ct][u][e] = (_Float16)(w - (float)w16);
+                }
+                const _Float16 o = (_Float16)1.f;
+                const h8_t ones = {o, o, o, o, o, o, o, o};
+                total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[ct][u], total[ct], 0, 0, 0);
+                if constexpr (SPLIT) total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[ct][u], total[ct], 0, 0, 0);
             }
-            const _Float16 o = (_Float16)1.f;
-            const h8_t ones = {o, o, o, o, o, o, o, o};
-            total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[ct], total[ct], 0, 0, 0);
-            if constexpr (SPLIT) total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[ct], total[ct], 0, 0, 0);
         }
         if constexpr (!F16) {
             if (vb != 0) {
-                const uint32_t vbw[2] = {mark_word(mark, 2, 0), mark_word(mark, 2, 1)};
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const _Float16 up = (vbw[e / 4] >> mark_bit(4 * g + e % 4)) & 1u ? (_Float16)16.f : (_Float16)1.f;
-                        ph[ct][e] *= up;
-                        if constexpr (SPLIT) pl[ct][e] *= up;
+                    for (int u = 0; u < KT / 2; ++u) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const _Float16 up = (tile_marks(vb, 2 * u + e / 4) >> (4 * g + e % 4)) & 1u ? (_Float16)16.f : (_Float16)1.f;
+                            ph[ct][u][e] *= up;
+                            if constexpr (SPLIT) pl[ct][u][e] *= up;
+                        }
                     }
                 }
             }
@@ -624,97 +624,56 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 
         // ---- O^T += V^T P^T ----
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            h8_t v[2], vl[VLO ? 2 : 1];  // of tile a: 4 tokens of d-tile 2i and of 2i + 1
+        for (int u = 0; u < KT / 2; ++u) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                v[a] = *reinterpret_cast<const h8_t*>(st + (2 + a) * kTileB + i * 1024 + lane * 16);
-                if constexpr (VLO) vl[a] = *reinterpret_cast<const h8_t*>(low + (2 + a) * kTileB + i * 1024 + lane * 16);
-            }
+            for (int i = 0; i < NQ; ++i) {
+                h8_t v[2], vl[VLO ? 2 : 1];  // of tile 2u + a: 4 tokens of d-tile 2i and of 2i + 1
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const h8_t w = o ? __builtin_shufflevector(v[0], v[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 8, 9, 10, 11);
-                h8_t wl;
-                if constexpr (VLO) wl = o ? __builtin_shufflevector(vl[0], vl[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(vl[0], vl[1], 0, 1, 2, 3, 8, 9, 10, 11);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    f4_t& c = acc[ct][2 * i + o];
-                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, ph[ct], c, 0, 0, 0);
-                    if constexpr (SPLIT) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, pl[ct], c, 0, 0, 0);
-                    if constexpr (VLO) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, ph[ct], c, 0, 0, 0);
+                for (int a = 0; a < 2; ++a) {
+                    const int at = (KT + 2 * u + a) * kTileB + i * 1024 + lane * 16;
+                    v[a] = *reinterpret_cast<const h8_t*>(st + at);
+                    if constexpr (VLO) vl[a] = *reinterpret_cast<const h8_t*>(low + at);
                 }
-            }
-            if constexpr (CT > 1 && SPLIT) __builtin_amdgcn_sched_barrier(0);
-        }
-        settle();
-        if (masked && (mark_word(mark, 3, 0) | mark_word(mark, 3, 1)) != 0) {
-            // rare: what is not finite reaches the rows that see it.  +inf where a visible value is +inf or NaN, and
-            // -inf where one is -inf or NaN (both: NaN), counted by products of ones; values from memory
-            const Entries e = fetch(step);
-            // (lane numbers that the compiler does not know to be loop invariants: it would keep this branch's
-            // addresses in registers all along)
-            int nn = n, gg = g;
-            asm volatile("" : "+v"(nn), "+v"(gg));
-            kernel_args* late = late_args();
-#pragma unroll 1
-            for (int a = 0; a < 2; ++a) {
-                const Where w0 = where(step, 0, e), w1 = where(step, 1, e);
-                const Where w = {a ? w1.bh : w0.bh, a ? w1.slot0 : w0.slot0, a ? w1.valid : w0.valid};
-                uint32_t seen[CT];
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) seen[ct] = sees(ct, a);
-#pragma unroll
-                for (int j = 0; j < NDT; ++j) {
-                    const uint32_t d = F16 ? 32 * (j / 2) + 2 * nn + j % 2 : 16 * j + nn;
-                    h4_t plus, minus;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool in = 4 * gg + r < w.valid;
-                        const float v = in ? tree_value<DT, D>(late->v, late->vs, (uint32_t)P, w.bh, (uint32_t)(w.slot0 + 4 * gg + r), d) : 0.f;
-                        plus[r] = in && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                        minus[r] = in && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                    }
+                for (int o = 0; o < 2; ++o) {
+                    const h8_t w = o ? __builtin_shufflevector(v[0], v[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 8, 9, 10, 11);
+                    h8_t wl;
+                    if constexpr (VLO) wl = o ? __builtin_shufflevector(vl[0], vl[1], 4, 5, 6, 7, 12, 13, 14, 15) : __builtin_shufflevector(vl[0], vl[1], 0, 1, 2, 3, 8, 9, 10, 11);
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) {
-                        h4_t vis;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) vis[r] = (seen[ct] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
-                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
-                        const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
-                        const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
-                        settle();
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
-                            acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
-                        }
+                        f4_t& c = acc[ct][2 * i + o];
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, ph[ct][u], c, 0, 0, 0);
+                        if constexpr (SPLIT) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, pl[ct][u], c, 0, 0, 0);
+                        if constexpr (VLO) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, ph[ct][u], c, 0, 0, 0);
                     }
                 }
+                if constexpr (CT > 1 && SPLIT) __builtin_amdgcn_sched_barrier(0);
             }
         }
+        settle();
+        if (masked && marks_of(mark, 3) != 0) wild = true;
     };
 
     // Step s's loads are in slot (s - lo) % (AHEAD + 1); those of its wave have landed once no more than
     // the loads of the AHEAD - 1 steps after it are on their way.
+    auto mine = [&](const int tokens) { return (tokens >> (5 * my_tile)) & 31; };
     wait_loads<(AHEAD - 1) * kLoads>();
-    prepare(lo, (held[0] >> (8 * my_tile)) & 0xff, 0, 0, 0);
+    prepare(lo, mine(held[0]), 0, 0, 0);
     barrier_lds();
     int slot = 0, mark = 0;
     for (int step = lo; step < hi; ++step) {
         const int next = slot == AHEAD ? 0 : slot + 1;
-        const Entries e = ahead;
-        ahead = fetch(step + AHEAD + 1);
-        held[AHEAD] = load_step(step + AHEAD, slot == 0 ? AHEAD : slot - 1, e);
-        compute(step, F16 ? slot : 0, mark, held[0] & 0xff, held[0] >> 8);
+        held[AHEAD] = load_step(step + AHEAD, slot == 0 ? AHEAD : slot - 1);
+        compute(step, F16 ? slot : 0, mark, held[0]);
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s) held[s] = held[s + 1];
         wait_loads<(AHEAD - 1) * kLoads>();
         if constexpr (F16) {
             mark ^= 1;
-            prepare(step + 1, (held[0] >> (8 * my_tile)) & 0xff, next, mark, 0);
+            prepare(step + 1, mine(held[0]), next, mark, 0);
         } else {
             barrier_lds();  // (every wave has read this step's rows)
-            prepare(step + 1, (held[0] >> (8 * my_tile)) & 0xff, 0, 0, next);
+            prepare(step + 1, mine(held[0]), 0, 0, next);
         }
         barrier_lds();
         slot = next;
@@ -724,6 +683,47 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 
     kernel_args* late = late_args();
     const int group = (int)late->group;
+    if (wild) {
+        // What is not finite reaches the rows that see it: +inf where a visible value is +inf or NaN, and -inf where
+        // one is -inf or NaN (both: NaN), counted by products of ones; values from memory.
+        for (int tile = first_tile(max(lo, tp.prefix_steps)); tile < min(first_tile(hi), tp.tiles); ++tile) {
+            const int row = tree_block_of(magic, shift, tile), slot0 = tile * kTile - row * P;
+            const int entry = as_const(tables)[row];
+            if (entry < 0 || (uint32_t)entry >= num_blocks) continue;
+            const size_t bh = (size_t)entry * hkv + h;
+            const int valid = min(min(kTile, sp.end - tile * kTile), used ? max(0, as_const(used)[row] - slot0) : kTile);
+            uint32_t seen[CT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) seen[ct] = sees(ct, tile, valid);
+#pragma unroll
+            for (int j = 0; j < NDT; ++j) {
+                const uint32_t d = F16 ? 32 * (j / 2) + 2 * n + j % 2 : 16 * j + n;
+                h4_t plus, minus;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool in = 4 * g + r < valid;
+                    const float v = in ? tree_value<DT, D>(late->v, late->vs, (uint32_t)P, bh, (uint32_t)(slot0 + 4 * g + r), d) : 0.f;
+                    plus[r] = in && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                    minus[r] = in && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    h4_t vis;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) vis[r] = (seen[ct] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
+                    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                    const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
+                    const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
+                    settle();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
+                        acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
+                    }
+                }
+            }
+        }
+    }
     const bool whole = tp.count == 1;
     const size_t state = ((size_t)b * (late->hkv * late->col_groups) + item) * late->parts + part;
 #pragma unroll
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 template <int DT, int D, typename IO, int CT, int W>
 void launch(const TreeParams& p, hipStream_t s) {
     hipLaunchKernelGGL((tree_wide<DT, D, IO, CT, W>), dim3(p.hkv * p.col_groups * p.parts, p.batch), dim3(W * 64), 0, s, p);
-    if (p.parts > 1) launch_merge<DT, D, IO>(p, W * CT, s);
+    if (p.parts > 1) launch_merge<DT, D, IO, wide_step_tiles(SPLIT_IO<IO>, CT)>(p, W * CT, s);
 }
 
 template <int DT, int D, typename IO>

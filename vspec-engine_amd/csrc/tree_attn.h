@@ -65,10 +65,11 @@ __device__ __forceinline__ uint64_t tree_bits(const TreeParams& p, uint32_t b, i
     return i < len ? m & all : 0;
 }
 
-// Element e of the value row in `slot` of (block, head) bh of an f16 or int4 pool, where it may be other than
-// finite (of an int4 pool: else 0, a code times a finite scale is finite).
+// Element e of the value row in `slot` of (block, head) bh where it may be other than finite
+// (of an int4 pool: else 0, a code times a finite scale is finite).
 template <int DT, int D>
 __device__ __forceinline__ float tree_value(const uint8_t* values, const uint16_t* scales, uint32_t P, size_t bh, uint32_t slot, uint32_t e) {
+    if constexpr (DT == VSPEC_KV_F32) return reinterpret_cast<const float*>(values)[(bh * P + slot) * D + e];
     if constexpr (DT == VSPEC_KV_F16) return half_bits_to_float(reinterpret_cast<const uint16_t*>(values)[f16_v_index(bh, P, D, slot, e)]);
     uint32_t high;
     const uint8_t c = values[int4_v_byte(bh, P, D, slot, e, &high)];
@@ -130,5 +131,10 @@ void launch_tree_wide_int4_d128(const TreeParams& p, int32_t io, uint32_t ct, hi
 // 16-token tiles of a step
 constexpr int wide_step_tiles(bool f32_rows, int ct) { return f32_rows || ct > 1 ? 2 : 4; }
 constexpr int tree_step_tiles(int dtype) { return dtype == VSPEC_KV_F32 ? 1 : 2; }
+// Workgroups of tree_mfma.hip that a CU holds.  Two hide each other's waits, where 256 registers a
+// lane hold K, V, q and the output without spilling more than a few.
+constexpr int tree_cu_groups(int dtype, int d, bool f32_rows, int ct) {
+    return ct == 1 || d == 64 || dtype == VSPEC_KV_F32 || (dtype == VSPEC_KV_F16 && !f32_rows) ? 2 : 1;
+}
 
 }  // namespace vkv

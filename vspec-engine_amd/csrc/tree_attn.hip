@@ -74,7 +74,7 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype));
     const uint64_t steps = (bound + per - 1) / per;
     const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups * d->batch;
-    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : 2) : 1);
+    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : 2) : tree_cu_groups(d->kv.dtype, d->kv.head_dim, f32_rows, pl.ct));
     uint64_t parts = items ? slots / items : 1;
     const uint64_t most = pl.wide ? steps / 4 : steps * pl.col_waves / 8;  // two steps a wave
     if (parts > most) parts = most;

@@ -47,11 +47,6 @@ __device__ __forceinline__ void settle() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <bool B>
-struct BoolTag {
-    static constexpr bool value = B;
-};
-
 constexpr uint32_t kBigScale = 0x6C00u;  // 2^12: a code times it may pass f16's range
 
 // fp16 scales of group c of the lane's tokens 4g + 2e and 4g + 2e + 1 (token r's halves start at word r NQ / 2)
@@ -71,6 +66,54 @@ __device__ __forceinline__ void int4_values(uint32_t codes, const h2_t (&scale)[
     if constexpr (LOW) {
         el = __builtin_shufflevector(__builtin_elementwise_fma(q[0], scale[0], -e0), __builtin_elementwise_fma(q[2], scale[1], -e1), 0, 1, 2, 3);
         ol = __builtin_shufflevector(__builtin_elementwise_fma(q[1], scale[0], -o0), __builtin_elementwise_fma(q[3], scale[1], -o1), 0, 1, 2, 3);
+    }
+}
+
+// After the tokens' loop, and rarely: what is not finite among the nodes' values reaches the rows that see it.  The
+// loop took it as zeros, for in its products 0 * inf would have reached the others.  +inf where a visible value is
+// +inf or NaN, and -inf where one is -inf or NaN (both: NaN), counted by products of ones over tiles [first, last).
+template <int DT, int D, int CT, typename SEES>
+__device__ __forceinline__ void add_wild(const int32_t* tables, const int32_t* used, uint32_t num_blocks, uint32_t hkv, uint32_t h, int P, uint32_t magic,
+                                         uint32_t shift, const TreeSpan& sp, int lane, int first, int last, SEES sees, f4_t (&acc)[CT][D / 16]) {
+    kernel_args* late = late_args();
+    const int g = lane >> 4, n = lane & 15;
+    for (int tile = first; tile < last; ++tile) {
+        const int row = tree_block_of(magic, shift, tile), slot0 = tile * kTile - row * P;
+        const int entry = as_const(tables)[row];
+        if (entry < 0 || (uint32_t)entry >= num_blocks) continue;
+        const size_t bh = (size_t)entry * hkv + h;
+        const int valid = min(min(kTile, sp.end - tile * kTile), used ? max(0, as_const(used)[row] - slot0) : kTile);
+        uint32_t seen[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) seen[ct] = sees(ct, tile, valid);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            // the element of V operand j in this lane
+            const uint32_t d = DT == VSPEC_KV_F16 ? 32 * (j / 2) + 2 * n + j % 2 : DT == VSPEC_KV_INT4 ? 16 * j + n : 64 * (j / 4) + 4 * n + j % 4;
+            h4_t plus, minus;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = 4 * g + r < valid;
+                const float v = in ? tree_value<DT, D>(late->v, late->vs, (uint32_t)P, bh, (uint32_t)(slot0 + 4 * g + r), d) : 0.f;
+                plus[r] = in && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+                minus[r] = in && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                h4_t vis;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vis[r] = (seen[ct] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
+                const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
+                const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
+                settle();
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
+                    acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
+                }
+            }
+        }
     }
 }
 

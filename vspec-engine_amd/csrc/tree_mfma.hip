@@ -51,7 +51,7 @@ struct Tile<VSPEC_KV_F32, D> {
 };
 
 template <int DT, int D, typename IO, int CT>
-__global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
+__global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) void tree_attention(TreeParams p) {
     constexpr bool F32 = DT == VSPEC_KV_F32;
     constexpr bool SPLIT = sizeof(IO) == 4 && !F32;      // q and p in two f16 parts
     constexpr bool VLO = SPLIT && DT == VSPEC_KV_INT4;   // K and V in two f16 parts
@@ -80,51 +80,80 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
     if (threadIdx.x < p.nodes) bits_sh[threadIdx.x] = tree_bits(p, b, threadIdx.x, sp.len);
     __syncthreads();
 
-    const int P = (int)p.block_tokens;
+    const int P = (int)own_scalar(p.block_tokens);
+    const int32_t* const tables = own_scalar(p.block_tables + (size_t)b * p.max_blocks);
+    const int32_t* const used = own_scalar(p.block_used ? p.block_used + (size_t)b * p.max_blocks : nullptr);
+    const uint8_t* const kdata = own_scalar(p.k);
+    const uint8_t* const vdata = own_scalar(p.v);
+    const uint16_t* const kscales = own_scalar(p.ks);
+    const uint16_t* const vscales = own_scalar(p.vs);
+    const uint32_t num_blocks = own_scalar(p.num_blocks), hkv = own_scalar(p.hkv);
+    const uint32_t magic = own_scalar(p.block_magic), shift = own_scalar(p.block_shift);
+    const float alpha = own_scalar(p.alpha), input_clip = own_scalar(p.input_clip);
 
     // ---- tiles ----
-    // Loads go out whatever the entry (one that names no block reads block 0) and hold as many
-    // valid tokens as the call returns.
-    auto load_tile = [&](const int tile, const bool in, T& f) -> int {
-        const size_t row = (size_t)b * p.max_blocks + (in ? tree_block_of(p.block_magic, p.block_shift, tile) : 0);
-        const int entry = as_const(p.block_tables)[row];
-        const bool ok = in && entry >= 0 && (uint32_t)entry < p.num_blocks;
-        const size_t bh = (size_t)(ok ? entry : 0) * p.hkv + h;
-        const int slot0 = in ? tile * kTile - tree_block_of(p.block_magic, p.block_shift, tile) * P : 0;
+    // The tiles of this wave's next 64 / NT steps, a lane each: where a tile lies (token index in the pool), its
+    // slot in the block and how many tokens it holds (0: its loads read block 0).
+    auto first_tile = [&](const int step) { return step < tp.prefix_steps ? NT * step : tp.prefix_tiles + NT * (step - tp.prefix_steps); };
+    size_t t_token = 0;
+    int t_info = 0;  // slot0 << 5 | tokens
+    auto look_up = [&](const int first) {
+        const int step = first + lane / NT * token_waves, tile = first_tile(step) + lane % NT;
+        const bool in = step < hi && tile < (step < tp.prefix_steps ? tp.prefix_tiles : tp.tiles);
+        const int row = in ? tree_block_of(magic, shift, tile) : 0;
+        const int entry = tables[row];
+        const int room = used ? used[row] : P;
+        const bool ok = in && entry >= 0 && (uint32_t)entry < num_blocks;
+        const int slot0 = ok ? tile * kTile - row * P : 0;
+        t_token = ((size_t)(ok ? entry : 0) * hkv + h) * P + slot0;
+        t_info = slot0 << 5 | (ok ? min(min(kTile, sp.end - tile * kTile), max(0, room - slot0)) : 0);
+    };
+    auto load_k = [&](const size_t token, const int slot0, T& f) {
         if constexpr (DT == VSPEC_KV_F16) {
-            const uint4* kr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(p.k) + (bh * P + slot0 + n) * D + 8 * g);
-            const uint4* vr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(p.v) + f16_v_index(bh, P, D, slot0 + 4 * g, 2 * n));
+            const uint4* kr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(kdata) + (token + n) * D + 8 * g);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) f.k[i] = kr[4 * i];
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) f.v[i] = vr[16 * i];
         } else if constexpr (DT == VSPEC_KV_INT4) {
-            const uint32_t* kr = reinterpret_cast<const uint32_t*>(p.k + (bh * P + slot0 + n) * (D / 2)) + g * NQ;
-            const uint32_t* vr = reinterpret_cast<const uint32_t*>(p.v + bh * ((size_t)P * D / 2) + (size_t)slot0 * (D / 2)) + (16 * g + n) * NQ;
-            const uint32_t* vs = reinterpret_cast<const uint32_t*>(p.vs + (bh * P + slot0 + 4 * g) * NQ);
+            const uint32_t* kr = reinterpret_cast<const uint32_t*>(kdata + (token + n) * (D / 2)) + g * NQ;
             if constexpr (NQ == 4) {
-                const uint4 a = *reinterpret_cast<const uint4*>(kr), c = *reinterpret_cast<const uint4*>(vr);
-                const uint4 s0 = reinterpret_cast<const uint4*>(vs)[0], s1 = reinterpret_cast<const uint4*>(vs)[1];
+                const uint4 a = *reinterpret_cast<const uint4*>(kr);
                 f.k[0] = a.x, f.k[1] = a.y, f.k[2] = a.z, f.k[3] = a.w;
-                f.v[0] = c.x, f.v[1] = c.y, f.v[2] = c.z, f.v[3] = c.w;
-                f.vs[0] = s0.x, f.vs[1] = s0.y, f.vs[2] = s0.z, f.vs[3] = s0.w;
-                f.vs[4] = s1.x, f.vs[5] = s1.y, f.vs[6] = s1.z, f.vs[7] = s1.w;
             } else {
-                const uint2 a = *reinterpret_cast<const uint2*>(kr), c = *reinterpret_cast<const uint2*>(vr);
-                const uint4 s0 = *reinterpret_cast<const uint4*>(vs);
+                const uint2 a = *reinterpret_cast<const uint2*>(kr);
                 f.k[0] = a.x, f.k[1] = a.y;
-                f.v[0] = c.x, f.v[1] = c.y;
-                f.vs[0] = s0.x, f.vs[1] = s0.y, f.vs[2] = s0.z, f.vs[3] = s0.w;
             }
-            f.ks = p.ks[int4_ks_index(bh, NQ, P, slot0 + n, (uint32_t)(g * NQ) / 4u)];
+            f.ks = kscales[(token - slot0) * NQ + (size_t)((g * NQ) / 4) * P + slot0 + n];
         } else {
-            const float* kr = reinterpret_cast<const float*>(p.k) + (bh * P + slot0 + n) * D + 4 * g;
-            const float* vr = reinterpret_cast<const float*>(p.v) + (bh * P + slot0 + 4 * g) * D + 4 * n;
+            const float* kr = reinterpret_cast<const float*>(kdata) + (token + n) * D + 4 * g;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const float4 w = *reinterpret_cast<const float4*>(kr + 16 * i);
                 f.k[4 * i] = w.x, f.k[4 * i + 1] = w.y, f.k[4 * i + 2] = w.z, f.k[4 * i + 3] = w.w;
             }
+        }
+    };
+    auto load_v = [&](const size_t token, T& f) {
+        if constexpr (DT == VSPEC_KV_F16) {
+            const uint4* vr = reinterpret_cast<const uint4*>(reinterpret_cast<const _Float16*>(vdata) + token * D + g * 4 * D + 8 * n);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) f.v[i] = vr[16 * i];
+        } else if constexpr (DT == VSPEC_KV_INT4) {
+            const uint32_t* vr = reinterpret_cast<const uint32_t*>(vdata + token * (D / 2)) + (16 * g + n) * NQ;
+            const uint4* vs = reinterpret_cast<const uint4*>(vscales + (token + 4 * g) * NQ);
+            if constexpr (NQ == 4) {
+                const uint4 c = *reinterpret_cast<const uint4*>(vr);
+                f.v[0] = c.x, f.v[1] = c.y, f.v[2] = c.z, f.v[3] = c.w;
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2*>(vr);
+                f.v[0] = c.x, f.v[1] = c.y;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const uint4 w = vs[i];
+                f.vs[4 * i] = w.x, f.vs[4 * i + 1] = w.y, f.vs[4 * i + 2] = w.z, f.vs[4 * i + 3] = w.w;
+            }
+        } else {
+            const float* vr = reinterpret_cast<const float*>(vdata) + (token + 4 * g) * D + 4 * n;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -134,37 +163,39 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                 }
             }
         }
-        int cap = ok ? kTile : 0;
-        if (p.block_used) cap = ok ? used_cap(as_const(p.block_used)[row], slot0) : 0;
-        return min(cap, max(sp.end - tile * kTile, 0));
     };
-    struct Step {
-        T t[NT];
-        int valid[NT];
-        int tile;  // the first one
+    struct Where {
+        size_t token[NT];
+        int slot0[NT], valid[NT];
     };
-    // prefix steps hold whole tiles of the prefix, tree steps those from the first that holds a node
-    auto load = [&](int step, const int limit, Step& s) {
-        step = __builtin_amdgcn_readfirstlane(step);
-        const bool prefix = step < tp.prefix_steps;
-        s.tile = prefix ? step * NT : tp.prefix_tiles + (step - tp.prefix_steps) * NT;
-        const int last = prefix ? tp.prefix_tiles : tp.tiles;
+    int at_lane = 0;  // of the next step's first tile in the table
+    auto where = [&](const int step, Where& w) {
+        if (at_lane == 64) {
+            look_up(step);
+            at_lane = 0;
+        }
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
-            const bool in = step < limit && s.tile + a < last;
-            s.valid[a] = load_tile(s.tile + a, in, s.t[a]);
-            if (!in) s.valid[a] = 0;
+            const uint32_t t0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)t_token, at_lane + a);
+            const uint32_t t1 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(t_token >> 32), at_lane + a);
+            const int info = __builtin_amdgcn_readlane(t_info, at_lane + a);
+            w.token[a] = (size_t)t1 << 32 | t0;
+            w.slot0[a] = info >> 5;
+            w.valid[a] = info & 31;
         }
+        at_lane += NT;
     };
 
-    // this wave's prefix steps and its tree steps (which come first: their loads share the round trip)
-    Step ring[2];
-    const int prefix_hi = min(hi, tp.prefix_steps);
+    Where now;
+    T tile[NT];
     int step = lo + tw;
-    int tree_step = step >= tp.prefix_steps ? step : step + (tp.prefix_steps - step + token_waves - 1) / token_waves * token_waves;
-    const bool has_tree = tree_step < hi;
-    if (has_tree) load(tree_step, hi, ring[1]);
-    load(step, prefix_hi, ring[0]);
+    look_up(step);
+    where(step, now);
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+        load_k(now.token[a], now.slot0[a], tile[a]);
+        load_v(now.token[a], tile[a]);
+    }
 
     // ---- q: columns of this wave ----
     // Column c is node c / group, head c % group of the kv head's.  The operands hold clip(q) 2^e
@@ -208,7 +239,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
         const float mean = sum * (1.0f / D);
 #pragma unroll
         for (int e = 0; e < E; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
-        const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+        const float th = fminf(fmaxf(1e-6f, alpha * sqrtf(add_rows(var) * (1.0f / D))), input_clip);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             x[e] = fminf(fmaxf(x[e], -th), th);
@@ -250,8 +281,22 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
         for (int j = 0; j < NDT; ++j) acc[ct][j] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto process = [&](auto tree_tag, Step& s) {
-        constexpr bool TREE = decltype(tree_tag)::value;
+    auto sees = [&](const int ct, const int tile, const int valid) -> uint32_t {
+        const int j0 = tile * kTile + 4 * g - sp.start;  // the node that the lane's first token is
+        const uint64_t mine = bits_sh[node[ct]];
+        const uint32_t seen = j0 <= -4 ? 15u
+                              : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
+                              : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
+        const int left = valid - 4 * g;
+        return seen & (left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u);
+    };
+    bool wild = false;  // V held what is not finite, among nodes
+
+    // K's registers take the next step's as soon as the scores are there, V's at the end.
+    auto process = [&](const int step, const Where& s, const Where& next) {
+        // a tile that holds nodes or fewer than 16 tokens
+        const bool masked = step >= tp.prefix_steps || s.valid[0] < kTile || s.valid[NT - 1] < kTile;
+        const int tile0 = first_tile(step);
         // ---- K operands, each key held to its own limit ----
         h8_t kh[F32 ? 1 : NT][NQ], kl[SPLIT ? NT : 1][NQ];
         bool low[NT];    // kl holds something
@@ -259,7 +304,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
         bool nans[NT];   // a key may be NaN
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
-            T& t = s.t[a];
+            T& t = tile[a];
             low[a] = VLO;
             kunit[a] = 1.f;
             nans[a] = F32;
@@ -271,7 +316,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                 const float mean = add_rows(sum) * (1.0f / D);
 #pragma unroll
                 for (int e = 0; e < D / 4; ++e) var = fmaf(t.k[e] - mean, t.k[e] - mean, var);
-                const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+                const float th = fminf(fmaxf(1e-6f, alpha * sqrtf(add_rows(var) * (1.0f / D))), input_clip);
 #pragma unroll
                 for (int e = 0; e < D / 4; ++e) t.k[e] = t.k[e] != t.k[e] ? t.k[e] : __builtin_amdgcn_fmed3f(t.k[e], -th, th);
             } else {
@@ -330,7 +375,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                 s2 = add_rows(s2);
                 const float mean1 = s1 * (1.0f / D), ex2 = s2 * (1.0f / D);
                 const float var1 = ex2 - mean1 * mean1;
-                const float th1 = fminf(fmaxf(1e-6f, p.alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), p.input_clip);
+                const float th1 = fminf(fmaxf(1e-6f, alpha * __builtin_amdgcn_sqrtf(fmaxf(var1, 0.f))), input_clip);
                 // the margins of the decode's screen; !(<=) also takes what is not finite
                 const bool flag = !(mx <= th1 * (1.0f - 0.0009765625f)) || var1 <= ex2 * 0.0009765625f;
                 const uint64_t any = __builtin_amdgcn_ballot_w64(flag && n < s.valid[a]);
@@ -359,7 +404,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                     const float mean = add_rows(sum) * (1.0f / D);
 #pragma unroll
                     for (int e = 0; e < 8 * NQ; ++e) var = fmaf(x[e] - mean, x[e] - mean, var);
-                    const float th = fminf(fmaxf(1e-6f, p.alpha * sqrtf(add_rows(var) * (1.0f / D))), p.input_clip);
+                    const float th = fminf(fmaxf(1e-6f, alpha * sqrtf(add_rows(var) * (1.0f / D))), input_clip);
                     const float down = large ? 0.0625f : 1.f;
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) {
@@ -388,7 +433,7 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                 f4_t c = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (F32) {
 #pragma unroll
-                    for (int e = 0; e < D / 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(s.t[a].k[e], qf[ct][e], c, 0, 0, 0);
+                    for (int e = 0; e < D / 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(tile[a].k[e], qf[ct][e], c, 0, 0, 0);
                 } else {
                     if constexpr (SPLIT) {
 #pragma unroll
@@ -416,6 +461,8 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
             }
         }
         settle();
+#pragma unroll
+        for (int a = 0; a < NT; ++a) load_k(next.token[a], next.slot0[a], tile[a]);
         if constexpr (DT == VSPEC_KV_INT4) {
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
@@ -425,41 +472,38 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
         }
 
         // ---- softmax of column n over the lane's tokens ----
-        uint32_t sees[TREE ? CT : 1][NT];  // bit r: the lane's token r is visible to its column
+        if (masked || nans[0] || nans[NT - 1]) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+                    const uint32_t seen = sees(ct, tile0 + a, s.valid[a]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x = sc[ct][a][r];
+                        // (a key with NaN is always flagged; the median would hide it)
+                        x = x != x ? x : __builtin_amdgcn_fmed3f(x, -clip[ct], clip[ct]);
+                        sc[ct][a][r] = (seen >> r) & 1u ? x : -INFINITY;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int a = 0; a < NT; ++a) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[ct][a][r] = __builtin_amdgcn_fmed3f(sc[ct][a][r], -clip[ct], clip[ct]);
+                }
+            }
+        }
         float top[CT];
         bool grown = false;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             top[ct] = -INFINITY;
 #pragma unroll
-            for (int a = 0; a < NT; ++a) {
-                f4_t x = sc[ct][a];
-                if (nans[a]) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = x[r] != x[r] ? x[r] : __builtin_amdgcn_fmed3f(x[r], -clip[ct], clip[ct]);
-                } else {
-                    // (a key with NaN is always flagged; the median would hide it)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_fmed3f(x[r], -clip[ct], clip[ct]);
-                }
-                if (TREE || s.valid[a] < kTile) {
-                    uint32_t seen = 15u;
-                    if constexpr (TREE) {
-                        const int j0 = (s.tile + a) * kTile + 4 * g - sp.start;  // the node that the lane's first token is
-                        const uint64_t mine = bits_sh[node[ct]];
-                        seen = j0 <= -4 ? 15u
-                               : j0 < 0 ? (uint32_t)(mine << -j0) | ((1u << -j0) - 1u)
-                               : j0 < 64 ? (uint32_t)(mine >> j0) : 0u;
-                    }
-                    const int held = s.valid[a] - 4 * g;
-                    seen &= held >= 4 ? 15u : held > 0 ? (1u << held) - 1u : 0u;
-                    if constexpr (TREE) sees[ct][a] = seen;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = (seen >> r) & 1u ? x[r] : -INFINITY;
-                }
-                sc[ct][a] = x;
-                top[ct] = fmaxf(top[ct], fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            }
+            for (int a = 0; a < NT; ++a) top[ct] = fmaxf(top[ct], fmaxf(fmaxf(sc[ct][a][0], sc[ct][a][1]), fmaxf(sc[ct][a][2], sc[ct][a][3])));
             grown = grown || top[ct] > limit[ct];
         }
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
@@ -498,39 +542,30 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
         // ---- V operands, O^T += V^T P^T ----
         // Slots without a token may hold any bits and become zeros.  In tiles that hold nodes so do values
         // that are not finite: in the products 0 * inf would reach the rows that do not see them.
-        bool wild[NT];
+        bool tree[NT];
+#pragma unroll
+        for (int a = 0; a < NT; ++a) tree[a] = (tile0 + a) * kTile + s.valid[a] > sp.start;
         if constexpr (F32) {
-            wild[0] = false;
-            float v[4][NDT];
-            bool mine = false;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool held = 4 * g + r < s.valid[0];
-#pragma unroll
-                for (int j = 0; j < NDT; ++j) {
-                    v[r][j] = s.t[0].v[r][j];
-                    if constexpr (TREE) {
-                        const bool out = !(fabsf(v[r][j]) < INFINITY);
-                        mine = mine || (held && out);
-                        v[r][j] = held && !out ? v[r][j] : 0.f;
-                    }
-                }
-            }
-            if constexpr (TREE) {
-                wild[0] = __builtin_amdgcn_ballot_w64(mine) != 0;
-            } else if (s.valid[0] < kTile) {
+            if (masked) {
+                bool mine = false;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
+                    const bool held = 4 * g + r < s.valid[0];
 #pragma unroll
-                    for (int j = 0; j < NDT; ++j) v[r][j] = 4 * g + r < s.valid[0] ? v[r][j] : 0.f;
+                    for (int j = 0; j < NDT; ++j) {
+                        const bool out = tree[0] && !(fabsf(tile[0].v[r][j]) < INFINITY);
+                        mine = mine || (held && out);
+                        tile[0].v[r][j] = held && !out ? tile[0].v[r][j] : 0.f;
+                    }
                 }
+                wild = wild || __builtin_amdgcn_ballot_w64(mine) != 0;
             }
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
                 for (int j = 0; j < NDT; ++j) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][j], pf[ct][r], acc[ct][j], 0, 0, 0);
+                    for (int r = 0; r < 4; ++r) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile[0].v[r][j], pf[ct][r], acc[ct][j], 0, 0, 0);
                 }
             }
         } else {
@@ -548,43 +583,42 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                         for (int e = 0; e < 2; ++e) {
                             // in the products of scales of 2^12 and more a code may pass f16's range: they are left
                             // for a product of their own
-                            uint32_t w = int4_scale_pair<NQ>(s.t[a], c, e);
+                            uint32_t w = int4_scale_pair<NQ>(tile[a], c, e);
                             if (s.valid[a] < kTile) {
                                 w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
                             }
                             const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
                             mine_big = mine_big || max(lo16, hi16) >= kBigScale;
-                            mine = mine || max(lo16, hi16) >= 0x7C00u;
+                            mine = mine || (tree[a] && max(lo16, hi16) >= 0x7C00u);
                             w &= (lo16 < kBigScale ? 0xffffu : 0u) | (hi16 < kBigScale ? 0xffff0000u : 0u);
                             sp2[e] = __builtin_bit_cast(h2_t, w);
                         }
-                        int4_values<VLO>(s.t[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
+                        int4_values<VLO>(tile[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
                     }
-                    wild[a] = TREE && __builtin_amdgcn_ballot_w64(mine) != 0;
+                    wild = wild || __builtin_amdgcn_ballot_w64(mine) != 0;
                 }
                 big = __builtin_amdgcn_ballot_w64(mine_big) != 0;
             } else {
 #pragma unroll
                 for (int a = 0; a < NT; ++a) {
-                    wild[a] = false;
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
-                        vh[a][2 * i] = __builtin_bit_cast(h4_t, make_uint2(s.t[a].v[i].x, s.t[a].v[i].y));
-                        vh[a][2 * i + 1] = __builtin_bit_cast(h4_t, make_uint2(s.t[a].v[i].z, s.t[a].v[i].w));
+                        vh[a][2 * i] = __builtin_bit_cast(h4_t, make_uint2(tile[a].v[i].x, tile[a].v[i].y));
+                        vh[a][2 * i + 1] = __builtin_bit_cast(h4_t, make_uint2(tile[a].v[i].z, tile[a].v[i].w));
                     }
-                    if (TREE || s.valid[a] < kTile) {
+                    if (masked) {
                         bool mine = false;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const bool held = 4 * g + r < s.valid[a];
 #pragma unroll
                             for (int j = 0; j < NDT; ++j) {
-                                const bool out = TREE && !(fabsf((float)vh[a][j][r]) < INFINITY);
+                                const bool out = tree[a] && !(fabsf((float)vh[a][j][r]) < INFINITY);
                                 mine = mine || (held && out);
                                 vh[a][j][r] = held && !out ? vh[a][j][r] : (_Float16)0.f;
                             }
                         }
-                        wild[a] = __builtin_amdgcn_ballot_w64(mine) != 0;
+                        wild = wild || __builtin_amdgcn_ballot_w64(mine) != 0;
                     }
                 }
             }
@@ -609,16 +643,16 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                             h2_t sp2[2];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                uint32_t w = int4_scale_pair<NQ>(s.t[a], c, e);
+                                uint32_t w = int4_scale_pair<NQ>(tile[a], c, e);
                                 if (s.valid[a] < kTile) {
                                     w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
                                 }
                                 const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
-                                const bool l_in = lo16 >= kBigScale && (!TREE || lo16 < 0x7C00u), h_in = hi16 >= kBigScale && (!TREE || hi16 < 0x7C00u);
+                                const bool l_in = lo16 >= kBigScale && (!tree[a] || lo16 < 0x7C00u), h_in = hi16 >= kBigScale && (!tree[a] || hi16 < 0x7C00u);
                                 w &= (l_in ? 0xffffu : 0u) | (h_in ? 0xffff0000u : 0u);
                                 sp2[e] = __builtin_bit_cast(h2_t, w) * down;
                             }
-                            int4_values<VLO>(s.t[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
+                            int4_values<VLO>(tile[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
                         }
                     }
                     const _Float16 up = (_Float16)16.f;
@@ -637,70 +671,18 @@ __global__ __launch_bounds__(256, 1) void tree_attention(TreeParams p) {
                 }
             }
         }
-        if constexpr (TREE) {
-            // What is not finite reaches the rows that see it: +inf where a visible value is +inf or NaN,
-            // and -inf where one is -inf or NaN (both: NaN), counted by products of ones.
 #pragma unroll
-            for (int a = 0; a < NT; ++a) {
-                if (!wild[a]) continue;
-#pragma unroll
-                for (int j = 0; j < NDT; ++j) {
-                    h4_t plus, minus;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float v;
-                        if constexpr (F32) {
-                            v = s.t[a].v[r][j];
-                        } else if constexpr (DT == VSPEC_KV_F16) {
-                            const uint4 w = s.t[a].v[j / 2];
-                            const uint32_t half2 = j % 2 ? (r < 2 ? w.z : w.w) : (r < 2 ? w.x : w.y);
-                            v = half_bits_to_float((half2 >> (16 * (r % 2))) & 0xffffu);
-                        } else {
-                            const uint32_t sc16 = int4_scale_pair<NQ>(s.t[a], j / 2, r / 2) >> (16 * (r % 2)) & 0xffffu;
-                            h2_t q4[4];
-                            codes_to_f16(s.t[a].v[j / 2], q4);
-                            v = (sc16 & 0x7fffu) >= 0x7C00u ? (float)q4[j % 2 + 2 * (r / 2)][r % 2] * half_bits_to_float(sc16) : 0.f;
-                        }
-                        const bool held = 4 * g + r < s.valid[a];
-                        plus[r] = held && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                        minus[r] = held && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                    }
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        h4_t vis;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) vis[r] = (sees[ct][a] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
-                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
-                        const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
-                        const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
-                        settle();
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
-                            acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
-                        }
-                    }
-                }
-            }
-        }
+        for (int a = 0; a < NT; ++a) load_v(next.token[a], tile[a]);
     };
 
-    if (has_tree) {
-        for (;;) {
-            process(BoolTag<true>{}, ring[1]);
-            tree_step += token_waves;
-            if (tree_step >= hi) break;
-            load(tree_step, hi, ring[1]);
-        }
+    for (; step < hi; step += token_waves) {
+        Where next;
+        where(step + token_waves, next);
+        process(step, now, next);
+        now = next;
     }
-    for (; step < prefix_hi; step += 2 * token_waves) {
-        load(step + token_waves, prefix_hi, ring[1]);
-        process(BoolTag<false>{}, ring[0]);
-        load(step + 2 * token_waves, prefix_hi, ring[0]);
-        process(BoolTag<false>{}, ring[1]);
-    }
-
     settle();
+    if (wild) add_wild<DT, D, CT>(tables, used, num_blocks, hkv, h, P, magic, shift, sp, lane, first_tile(max(lo, tp.prefix_steps)), min(first_tile(hi), tp.tiles), sees, acc);
 
     // ---- join the token waves; the output, or the part's state ----
     const bool whole = tp.count == 1;

@@ -683,47 +683,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 
     kernel_args* late = late_args();
     const int group = (int)late->group;
-    if (wild) {
-        // What is not finite reaches the rows that see it: +inf where a visible value is +inf or NaN, and -inf where
-        // one is -inf or NaN (both: NaN), counted by products of ones; values from memory.
-        for (int tile = first_tile(max(lo, tp.prefix_steps)); tile < min(first_tile(hi), tp.tiles); ++tile) {
-            const int row = tree_block_of(magic, shift, tile), slot0 = tile * kTile - row * P;
-            const int entry = as_const(tables)[row];
-            if (entry < 0 || (uint32_t)entry >= num_blocks) continue;
-            const size_t bh = (size_t)entry * hkv + h;
-            const int valid = min(min(kTile, sp.end - tile * kTile), used ? max(0, as_const(used)[row] - slot0) : kTile);
-            uint32_t seen[CT];
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) seen[ct] = sees(ct, tile, valid);
-#pragma unroll
-            for (int j = 0; j < NDT; ++j) {
-                const uint32_t d = F16 ? 32 * (j / 2) + 2 * n + j % 2 : 16 * j + n;
-                h4_t plus, minus;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool in = 4 * g + r < valid;
-                    const float v = in ? tree_value<DT, D>(late->v, late->vs, (uint32_t)P, bh, (uint32_t)(slot0 + 4 * g + r), d) : 0.f;
-                    plus[r] = in && !(v < INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                    minus[r] = in && !(v > -INFINITY) ? (_Float16)1.f : (_Float16)0.f;
-                }
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    h4_t vis;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) vis[r] = (seen[ct] >> r) & 1u ? (_Float16)1.f : (_Float16)0.f;
-                    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
-                    const f4_t up = __builtin_amdgcn_mfma_f32_16x16x16f16(plus, vis, zero, 0, 0, 0);
-                    const f4_t dn = __builtin_amdgcn_mfma_f32_16x16x16f16(minus, vis, zero, 0, 0, 0);
-                    settle();
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        acc[ct][j][r] += up[r] > 0.f ? INFINITY : 0.f;
-                        acc[ct][j][r] += dn[r] > 0.f ? -INFINITY : 0.f;
-                    }
-                }
-            }
-        }
-    }
+    if (wild) add_wild<DT, D, CT>(tables, used, num_blocks, hkv, h, P, magic, shift, sp, lane, first_tile(max(lo, tp.prefix_steps)), min(first_tile(hi), tp.tiles), sees, acc);
     const bool whole = tp.count == 1;
     const size_t state = ((size_t)b * (late->hkv * late->col_groups) + item) * late->parts + part;
 #pragma unroll

@@ -23,13 +23,14 @@ struct TreeParams {
     float alpha;       // std-clamp alpha
     float logit_clip;  // 24 * log2(e) in 3-bit mode, +inf otherwise
     float input_clip;  // 16 in 3-bit mode, +inf otherwise
-    // work split: an item is (sequence, kv head, group of column tiles); its steps are cut into
-    // up to `parts` parts of at least part_steps steps, a workgroup each
-    uint32_t parts, part_steps;
+    // work split (tree_job): a row of the grid is a sequence or a part of one, for every kv head and group of column
+    // tiles.  slot_rows: rows that the card holds at once (0: rows are sequences); min_units: least units of a part
+    uint32_t rows, slot_rows, min_units;
     uint32_t col_groups;  // of col_waves * CT tiles of 16 columns
     uint32_t col_waves;   // waves of a workgroup side by side over columns: 1, 2 or 4
-    float* part_acc;      // [item][part][column tile][D/16][lane][4]
-    float* part_ml;       // [item][part][column tile][16][2]: reference point (log2 units), sum
+    int4* plan;           // [0]: x sequences are in parts; [1 + i]: the ith of them, its parts, their first state
+    float* part_acc;      // [state][item][column tile][D/16][lane][4]; item: column group, kv head
+    float* part_ml;       // [state][item][column tile][16][2]: reference point (log2 units), sum
 };
 
 // The table entry of a tile, tile / (tiles of a block), as a product: tiles are below 2^27, and with 2^(s-1) <
@@ -47,16 +48,17 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 struct TreeSpan {
     int start, len, end;  // end: slots that the table holds of both
 };
-__device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, uint32_t b) {
+__device__ __forceinline__ TreeSpan make_span(const TreeParams& p, int start, int len) {
     const int cap = (int)min((uint64_t)p.max_blocks * p.block_tokens, (uint64_t)0x7fffff00u);
     TreeSpan s;
-    s.start = min(max(as_const(p.start_pos)[b], 0), cap);
-    s.len = p.tree_lens ? min(max(as_const(p.tree_lens)[b], 0), (int)p.nodes) : (int)p.nodes;
+    s.start = min(max(start, 0), cap);
+    s.len = min(max(len, 0), (int)p.nodes);
     s.end = min(s.start + s.len, cap);
-    s.start = uniform(s.start);
-    s.len = uniform(s.len);
-    s.end = uniform(s.end);
     return s;
+}
+__device__ __forceinline__ TreeSpan tree_span(const TreeParams& p, uint32_t b) {
+    const TreeSpan s = make_span(p, as_const(p.start_pos)[b], p.tree_lens ? as_const(p.tree_lens)[b] : (int)p.nodes);
+    return {uniform(s.start), uniform(s.len), uniform(s.end)};
 }
 // Bits of the nodes that node i of sequence b sees.
 __device__ __forceinline__ uint64_t tree_bits(const TreeParams& p, uint32_t b, int i, int len) {
@@ -78,21 +80,132 @@ __device__ __forceinline__ float tree_value(const uint8_t* values, const uint16_
 }
 
 // A sequence's steps of NT tiles: first the tiles that hold prefix alone, then those from the first
-// node's on.  Part i of them begins at step i * chunk.
-struct TreeParts {
-    int tiles, prefix_tiles, prefix_steps;
-    int steps, count, chunk;
+// node's on.
+struct TreeSteps {
+    int tiles, prefix_tiles, prefix_steps, steps;
 };
 template <int NT>
-__device__ __forceinline__ TreeParts tree_parts(const TreeParams& p, const TreeSpan& s) {
-    TreeParts r;
+__device__ __forceinline__ TreeSteps tree_steps(const TreeSpan& s) {
+    TreeSteps r;
     r.tiles = s.len ? (s.end + kTile - 1) / kTile : 0;  // (no nodes: nothing to read)
     r.prefix_tiles = min(s.start / kTile, r.tiles);
     r.prefix_steps = (r.prefix_tiles + NT - 1) / NT;
     r.steps = r.prefix_steps + (r.tiles - r.prefix_tiles + NT - 1) / NT;
-    const int most = max(1, min((int)p.parts, (r.steps + (int)p.part_steps - 1) / (int)p.part_steps));
-    r.chunk = uniform(max(1, (r.steps + most - 1) / most));
-    r.count = uniform(max(1, (r.steps + r.chunk - 1) / r.chunk));
+    return r;
+}
+
+// Inclusive prefix sums over the wave.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
+// What a row of the grid does: steps [lo, hi) of sequence b (< 0: nothing).
+//
+// The lengths are on the device, so the rows are dealt out there, by every wave for itself.  With `units` the steps
+// of a sequence in units of `unit`, sequence b gets ceil(units_b / c) rows: c is the mean load of a row that the
+// card holds, or, where there are fewer sequences than those, the least c (or one near it) that gives no more rows
+// than that, so that the longest row is about as short as it can be.  A division by the longest sequence alone
+// took 159 us where this takes 103 (13 sequences of up to 9000 tokens, 27 nodes).
+constexpr uint32_t kMaxSlotRows = 256;  // and parts of a sequence
+constexpr int kPlanGroups = 4;
+constexpr uint32_t kPlanSequences = 64 * kPlanGroups;
+struct TreeJob {
+    int b, lo, hi;
+    int part, count;  // of the sequence's parts
+    int state;        // of its first part, where count > 1
+    int split;        // sequences before it that are in parts
+    TreeSpan span;
+};
+template <int NT>
+__device__ __forceinline__ TreeJob tree_job(const TreeParams& p, int row, int unit) {
+    TreeJob r;
+    r.b = row;
+    r.part = 0;
+    r.count = 1;
+    r.state = 0;
+    r.split = 0;
+    r.lo = 0;
+    if (p.slot_rows == 0) {
+        r.span = tree_span(p, (uint32_t)row);
+        r.hi = tree_steps<NT>(r.span).steps;
+        return r;
+    }
+    const int lane = threadIdx.x & 63, batch = (int)p.batch;
+    int units[kPlanGroups], steps[kPlanGroups];
+    TreeSpan span[kPlanGroups];
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanGroups; ++k) {
+        units[k] = 0;
+        if (64 * k < batch) {
+            const int b = 64 * k + lane, from = min(b, batch - 1);
+            span[k] = make_span(p, p.start_pos[from], p.tree_lens ? p.tree_lens[from] : (int)p.nodes);
+            steps[k] = tree_steps<NT>(span[k]).steps;
+            units[k] = b < batch ? max(1, (steps[k] + unit - 1) / unit) : 0;
+            sum += units[k];
+        }
+    }
+    auto parts = [&](const int k, const int c) -> int { return (int)((uint32_t)(units[k] + c - 1) / (uint32_t)c); };
+    auto rows_of = [&](const int c) -> int {
+        int x = 0;
+#pragma unroll
+        for (int k = 0; k < kPlanGroups; ++k) {
+            if (64 * k < batch) x += parts(k, c);
+        }
+        return __builtin_amdgcn_readlane(wave_scan(x), 63);
+    };
+    const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63), most = (int)p.rows;
+    auto up = [](const int x, const int by) -> int { return uniform((x + by - 1) / by); };
+    int c = max((int)p.min_units, up(total, (int)p.slot_rows));
+    if (rows_of(c) > most) {
+        int hi = most > batch ? max(c + 1, up(total, most - batch)) : total;  // that many are enough
+        while (c + 1 < hi) {
+            const int mid = c + (hi - c) / 2;
+            if (rows_of(mid) > most) c = mid;
+            else hi = mid;
+        }
+        c = hi;
+    }
+    int base = 0, state = 0, split = 0;
+    r.b = -1;
+#pragma unroll
+    for (int k = 0; k < kPlanGroups; ++k) {
+        if (64 * k >= batch) continue;
+        const int mine = parts(k, c), held = mine > 1 ? mine : 0;
+        const int rows = wave_scan(mine), states = wave_scan(held);
+        const int l = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(base + rows <= row));
+        const uint64_t in_parts = __builtin_amdgcn_ballot_w64(mine > 1);
+        if (l < 64 && r.b < 0) {
+            const int n = __builtin_amdgcn_readlane(mine, l), u = __builtin_amdgcn_readlane(units[k], l), all = __builtin_amdgcn_readlane(steps[k], l);
+            const int even = up(u, n);  // no part much longer than another
+            r.count = up(u, even);
+            r.part = row - (base + __builtin_amdgcn_readlane(rows, l) - n);
+            r.b = r.part < r.count ? 64 * k + l : batch;  // (batch: a row too many)
+            r.state = state + __builtin_amdgcn_readlane(states, l) - (n > 1 ? n : 0);
+            r.split = split + (int)__builtin_popcountll(in_parts & ((1ull << l) - 1));
+            r.lo = r.part * even * unit;
+            r.hi = min(r.lo + even * unit, all);
+            r.span = {__builtin_amdgcn_readlane(span[k].start, l), __builtin_amdgcn_readlane(span[k].len, l), __builtin_amdgcn_readlane(span[k].end, l)};
+        }
+        base += __builtin_amdgcn_readlane(rows, 63);
+        state += __builtin_amdgcn_readlane(states, 63);
+        split += (int)__builtin_popcountll(in_parts);
+    }
+    if (r.b >= batch) r.b = -1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {  // for tree_merge
+        if (row == 0) p.plan[0].x = split;
+        if (r.b >= 0 && r.part == 0 && r.count > 1) p.plan[1 + r.split] = make_int4(r.b, r.count, r.state, 0);
+    }
+    r.b = uniform(r.b);
+    r.lo = uniform(r.lo), r.hi = uniform(r.hi);
+    r.part = uniform(r.part), r.count = uniform(r.count), r.state = uniform(r.state);
+    r.span = {uniform(r.span.start), uniform(r.span.len), uniform(r.span.end)};
     return r;
 }
 

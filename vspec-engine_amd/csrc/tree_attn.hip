@@ -47,13 +47,13 @@ int check_tree(const VspecTreeAttnDesc* d) {
 }
 
 struct TreePlan {
-    uint32_t ct, col_waves, col_groups, parts, part_steps;
+    uint32_t ct, col_waves, col_groups, rows, slot_rows, min_units;
     bool wide;  // tree_wide.hip
-    size_t acc_floats, ws_bytes;
+    size_t plan_bytes, acc_floats, ws_bytes;
 };
 
-// Columns first: a wave holds up to 4 tiles of 16 columns and a workgroup up to 16, so that K and
-// V are read once for as many rows as the registers hold.  Then parts, as many as fill the card.
+// Columns first: a workgroup holds as many as K and V can be read once for.  Then rows of the grid
+// (tree_job): sequences, and parts of them where that shortens the longest row.
 TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     TreePlan pl = {};
     const uint32_t cols = d->num_nodes * (d->num_q_heads / d->kv.num_kv_heads);
@@ -71,22 +71,27 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
     if (bound > cap) bound = cap;
     const bool f32_rows = d->io_dtype == VSPEC_KV_F32;
-    const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype));
-    const uint64_t steps = (bound + per - 1) / per;
-    const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups * d->batch;
-    const uint64_t slots = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : 2) : tree_cu_groups(d->kv.dtype, d->kv.head_dim, f32_rows, pl.ct));
-    uint64_t parts = items ? slots / items : 1;
-    const uint64_t most = pl.wide ? steps / 4 : steps * pl.col_waves / 8;  // two steps a wave
-    if (parts > most) parts = most;
-    if (parts < 1) parts = 1;
-    if (parts > 256) parts = 256;
-    pl.part_steps = (uint32_t)((steps + parts - 1) / parts);
-    if (pl.part_steps < 1) pl.part_steps = 1;
-    pl.parts = (uint32_t)parts;
-    if (parts > 1) {
-        const size_t states = (size_t)(items * parts * pl.col_waves * pl.ct);
-        pl.acc_floats = states * d->kv.head_dim * 16;
-        pl.ws_bytes = (pl.acc_floats + states * 32) * sizeof(float);
+    // a unit: a step, or one of each of the waves that share a row's steps
+    const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype) * (4 / pl.col_waves));
+    pl.min_units = pl.wide ? 4 : 1;
+    const uint64_t batch = d->batch, units = (bound + per - 1) / per;
+    const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups;
+    const uint64_t wgs = (uint64_t)host_num_cus() * (pl.wide ? (pl.col_waves == 8 ? 1 : 2) : tree_cu_groups(d->kv.dtype, d->kv.head_dim, f32_rows, pl.ct));
+    uint64_t slots = wgs / items ? wgs / items : 1;
+    if (slots > kMaxSlotRows) slots = kMaxSlotRows;
+    uint64_t rows = slots > batch ? slots : slots + batch;
+    const uint64_t most = batch * ((units + pl.min_units - 1) / pl.min_units);
+    if (rows > most) rows = most;
+    pl.rows = (uint32_t)batch;
+    if (rows > batch && batch <= kPlanSequences && batch * (cap / per + 2) < 1u << 30) {
+        pl.rows = (uint32_t)rows;
+        pl.slot_rows = (uint32_t)slots;
+        // parts of sequences that have more than one: at most a row's mean load each, and one more for each sequence
+        const uint64_t states = rows < 2 * slots ? rows : 2 * slots;
+        const size_t state_tiles = (size_t)(states * items * pl.col_waves * pl.ct);
+        pl.plan_bytes = (1 + slots) * sizeof(int4);
+        pl.acc_floats = state_tiles * d->kv.head_dim * 16;
+        pl.ws_bytes = pl.plan_bytes + (pl.acc_floats + state_tiles * 32) * sizeof(float);
     }
     return pl;
 }
@@ -160,12 +165,14 @@ extern "C" int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc) {
             }
         }
     }
-    p.parts = pl.parts;
-    p.part_steps = pl.part_steps;
+    p.rows = pl.rows;
+    p.slot_rows = pl.slot_rows;
+    p.min_units = pl.min_units;
     p.col_groups = pl.col_groups;
     p.col_waves = pl.col_waves;
-    p.part_acc = (float*)ws;
-    p.part_ml = (float*)ws + pl.acc_floats;
+    p.plan = (int4*)ws;
+    p.part_acc = (float*)((uint8_t*)ws + pl.plan_bytes);
+    p.part_ml = p.part_acc + pl.acc_floats;
     hipStream_t s = (hipStream_t)desc->stream;
     const bool d128 = kv.head_dim == 128;
     switch (kv.dtype) {

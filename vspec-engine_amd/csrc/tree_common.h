@@ -117,43 +117,89 @@ __device__ __forceinline__ void add_wild(const int32_t* tables, const int32_t* u
     }
 }
 
-// The parts of one column tile of an item, cut in steps of NT tiles.
-template <int DT, int D, typename IO, int NT>
-__global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t tiles) {
+// Joins the parts of the sequences that have more than one.  A task is a column tile of an item: the parts' weights
+// through LDS, then four of the output's d-tiles, a wave each, or, of many parts, one d-tile that the waves share.
+// Each load is 1 KB whole, and what counts is how many are on their way: a workgroup to a column tile, with every
+// weight read again for each d-tile, took some 50 us for the 64 parts of 8 items where this takes 4.
+constexpr uint32_t kMergeShared = 8;  // parts from which the waves share
+template <int DT, int D, typename IO>
+__global__ __launch_bounds__(256) void tree_merge(TreeParams p, uint32_t tiles, uint32_t cuts) {
     constexpr int NDT = D / 16;
-    const uint32_t b = blockIdx.y, item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
-    const uint32_t h = item / p.col_groups, cg = item - h * p.col_groups;
-    const TreeSpan sp = tree_span(p, b);
-    const TreeParts tp = tree_parts<NT>(p, sp);
-    if (tp.count == 1) return;
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int c = (int)((cg * tiles + tile) * 16) + n;
-    const bool live = c < (int)(p.nodes * p.group);
-    const int i = c / (int)p.group;
-    const size_t slot0 = ((size_t)b * (p.hkv * p.col_groups) + item) * p.parts;
-    float top = -INFINITY, total = 0.f;
-    for (int t = 0; t < tp.count; ++t) top = fmaxf(top, p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2]);
-    for (int t = 0; t < tp.count; ++t) {
-        const float* ml = p.part_ml + (((slot0 + t) * tiles + tile) * 16 + n) * 2;
-        total += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
-    }
-    const bool empty = i >= sp.len || total == 0.f;
-    for (int j = (int)(threadIdx.x >> 6); j < NDT; j += 4) {
-        f4_t a = {0.f, 0.f, 0.f, 0.f};
-        for (int t = 0; t < tp.count; ++t) {
-            const float f = __builtin_amdgcn_exp2f(p.part_ml[(((slot0 + t) * tiles + tile) * 16 + n) * 2] - top);
-            a += reinterpret_cast<const f4_t*>(p.part_acc)[(((slot0 + t) * tiles + tile) * NDT + j) * 64 + lane] * f;
+    extern __shared__ float merge_sh[];  // [2][slot_rows][16]: weights (first: reference points), sums
+    __shared__ float red[16][16];
+    __shared__ f4_t joined[4][64];
+    const uint32_t items = p.hkv * p.col_groups, per = items * tiles * cuts;
+    const uint32_t tasks = (uint32_t)as_const(&p.plan->x)[0] * per;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+    const int row = threadIdx.x >> 4;  // parts row, row + 16, ...
+    float* const ref_sh = merge_sh + n;
+    float* const sum_sh = ref_sh + 16 * p.slot_rows;
+    const bool share = cuts == NDT;
+    for (uint32_t task = blockIdx.x; task < tasks; task += gridDim.x) {
+        const uint32_t split = task / per, rest = task - split * per;
+        const uint32_t place = rest / cuts, cut = rest - place * cuts;  // place: item, column tile
+        const uint32_t item = place / tiles, tile = place - item * tiles;
+        const uint32_t cg = item / p.hkv, h = item - cg * p.hkv;
+        const int4 plan = p.plan[1 + split];
+        const uint32_t b = (uint32_t)uniform(plan.x);
+        const int count = uniform(plan.y);
+        const TreeSpan sp = tree_span(p, b);
+        const size_t pitch = (size_t)items * tiles, first = (size_t)uniform(plan.z) * pitch + place;  // states of the parts
+        float top = -INFINITY, total = 0.f;
+        __syncthreads();  // (the task before has read its weights)
+        for (int t = row; t < count; t += 16) {
+            const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[(first + t * pitch) * 16 + n];
+            ref_sh[16 * t] = ml.x;
+            sum_sh[16 * t] = ml.y;
+            top = fmaxf(top, ml.x);
         }
-        if (!live) continue;
+        red[row][n] = top;
+        __syncthreads();
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, red[r][n]);
+        for (int t = row; t < count; t += 16) {
+            const float f = __builtin_amdgcn_exp2f(ref_sh[16 * t] - top);
+            ref_sh[16 * t] = f;
+            total = fmaf(sum_sh[16 * t], f, total);
+        }
+        __syncthreads();
+        red[row][n] = total;
+        __syncthreads();
+        total = 0.f;
+        for (int r = 0; r < 16; ++r) total += red[r][n];
+
+        const int j = share ? (int)cut : 4 * (int)cut + wave, step = share ? 4 : 1;
+        const f4_t* src = reinterpret_cast<const f4_t*>(p.part_acc) + (first * NDT + j) * 64 + lane;
+        f4_t a = {0.f, 0.f, 0.f, 0.f};
+        int t = share ? wave : 0;
+        for (; t + 7 * step < count; t += 8 * step) {
+            f4_t x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = src[(size_t)(t + u * step) * pitch * (NDT * 64)];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a += x[u] * ref_sh[16 * (t + u * step)];
+        }
+        for (; t < count; t += step) a += src[(size_t)t * pitch * (NDT * 64)] * ref_sh[16 * t];
+        if (share) {
+            joined[wave][lane] = a;
+            __syncthreads();
+            if (wave != 0) continue;
+            a = (joined[0][lane] + joined[1][lane]) + (joined[2][lane] + joined[3][lane]);
+        }
+        const int c = (int)((cg * tiles + tile) * 16) + n;
+        if (c >= (int)(p.nodes * p.group)) continue;
+        const int i = c / (int)p.group;
+        const bool empty = i >= sp.len || total == 0.f;
         IO* dst = reinterpret_cast<IO*>(p.out) + (((size_t)b * p.nodes + i) * p.hq + (size_t)h * p.group + (c - i * (int)p.group)) * D;
 #pragma unroll
         for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : a[r] / total);
     }
 }
 
-template <int DT, int D, typename IO, int NT>
+template <int DT, int D, typename IO>
 void launch_merge(const TreeParams& p, uint32_t tiles, hipStream_t s) {
-    hipLaunchKernelGGL((tree_merge<DT, D, IO, NT>), dim3(p.hkv * p.col_groups * tiles, p.batch), dim3(256), 0, s, p, tiles);
+    const uint32_t cuts = p.slot_rows >= kMergeShared * p.batch ? D / 16 : D / 64;
+    const uint64_t tasks = (uint64_t)min(p.batch, p.slot_rows) * p.hkv * p.col_groups * tiles * cuts;
+    hipLaunchKernelGGL((tree_merge<DT, D, IO>), dim3((uint32_t)min(tasks, (uint64_t)1024)), dim3(256), p.slot_rows * 32 * sizeof(float), s, p, tiles, cuts);
 }
 
 }  // namespace

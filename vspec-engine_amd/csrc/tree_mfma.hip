@@ -69,13 +69,13 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
     const int token_waves = 4 / (int)p.col_waves;
     const int cw = wave / token_waves, tw = wave - cw * token_waves;
 
-    const uint32_t b = blockIdx.y;
-    const uint32_t item = (uint32_t)uniform((int)(blockIdx.x / p.parts)), part = blockIdx.x - item * p.parts;
-    const uint32_t h = (uint32_t)uniform((int)(item / p.col_groups)), cg = item - h * p.col_groups;
-    const TreeSpan sp = tree_span(p, b);
-    const TreeParts tp = tree_parts<NT>(p, sp);
-    if ((int)part >= tp.count) return;
-    const int lo = (int)part * tp.chunk, hi = min(lo + tp.chunk, tp.steps);
+    const TreeJob job = tree_job<NT>(p, (int)blockIdx.y, token_waves);
+    if (job.b < 0) return;
+    const uint32_t b = (uint32_t)job.b, item = blockIdx.x;
+    const uint32_t cg = (uint32_t)uniform((int)(item / p.hkv)), h = item - cg * p.hkv;
+    const TreeSpan sp = job.span;
+    const TreeSteps tp = tree_steps<NT>(sp);
+    const int lo = job.lo, hi = job.hi;
 
     if (threadIdx.x < p.nodes) bits_sh[threadIdx.x] = tree_bits(p, b, threadIdx.x, sp.len);
     __syncthreads();
@@ -685,9 +685,9 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
     if (wild) add_wild<DT, D, CT>(tables, used, num_blocks, hkv, h, P, magic, shift, sp, lane, first_tile(max(lo, tp.prefix_steps)), min(first_tile(hi), tp.tiles), sees, acc);
 
     // ---- join the token waves; the output, or the part's state ----
-    const bool whole = tp.count == 1;
+    const bool whole = job.count == 1;
     const int tiles = (int)p.col_waves * CT;
-    const size_t slot = ((size_t)b * (p.hkv * p.col_groups) + item) * p.parts + part;
+    const size_t slot = (size_t)(job.state + job.part) * (p.hkv * p.col_groups) + item;
     auto finish = [&](const int ct, const int j, f4_t a, const float sum, const float ref) {
         const int tile = cw * CT + ct;
         if (!whole) {
@@ -741,14 +741,12 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
 
 template <int DT, int D, typename IO>
 void launch(const TreeParams& p, uint32_t ct, hipStream_t s) {
-    const dim3 grid(p.hkv * p.col_groups * p.parts, p.batch);
+    const dim3 grid(p.hkv * p.col_groups, p.rows);
     switch (ct) {
         case 1: hipLaunchKernelGGL((tree_attention<DT, D, IO, 1>), grid, dim3(256), 0, s, p); break;
         default: hipLaunchKernelGGL((tree_attention<DT, D, IO, 2>), grid, dim3(256), 0, s, p); break;
     }
-    if (p.parts > 1) {
-        launch_merge<DT, D, IO, tree_step_tiles(DT)>(p, p.col_waves * ct, s);
-    }
+    if (p.slot_rows) launch_merge<DT, D, IO>(p, p.col_waves * ct, s);
 }
 
 }  // namespace

@@ -70,13 +70,13 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
-    const uint32_t b = blockIdx.y;
-    const uint32_t item = (uint32_t)uniform((int)(blockIdx.x / p.parts)), part = blockIdx.x - item * p.parts;
-    const uint32_t h = (uint32_t)uniform((int)(item / p.col_groups)), cg = item - h * p.col_groups;
-    const TreeSpan sp = tree_span(p, b);
-    const TreeParts tp = tree_parts<KT>(p, sp);
-    if ((int)part >= tp.count) return;
-    const int lo = (int)part * tp.chunk, hi = min(lo + tp.chunk, tp.steps);
+    const TreeJob job = tree_job<KT>(p, (int)blockIdx.y, 1);
+    if (job.b < 0) return;
+    const uint32_t b = (uint32_t)job.b, item = blockIdx.x;
+    const uint32_t cg = (uint32_t)uniform((int)(item / p.hkv)), h = item - cg * p.hkv;
+    const TreeSpan sp = job.span;
+    const TreeSteps tp = tree_steps<KT>(sp);
+    const int lo = job.lo, hi = job.hi;
     if (threadIdx.x < 64) bits_sh[threadIdx.x] = threadIdx.x < p.nodes ? tree_bits(p, b, threadIdx.x, sp.len) : 0;
 
     const int P = (int)own_scalar(p.block_tokens);
@@ -684,8 +684,8 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     kernel_args* late = late_args();
     const int group = (int)late->group;
     if (wild) add_wild<DT, D, CT>(tables, used, num_blocks, hkv, h, P, magic, shift, sp, lane, first_tile(max(lo, tp.prefix_steps)), min(first_tile(hi), tp.tiles), sees, acc);
-    const bool whole = tp.count == 1;
-    const size_t state = ((size_t)b * (late->hkv * late->col_groups) + item) * late->parts + part;
+    const bool whole = job.count == 1;
+    const size_t state = (size_t)(job.state + job.part) * (late->hkv * late->col_groups) + item;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const int tile = wave * CT + ct;
@@ -715,8 +715,8 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 
 template <int DT, int D, typename IO, int CT, int W>
 void launch(const TreeParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((tree_wide<DT, D, IO, CT, W>), dim3(p.hkv * p.col_groups * p.parts, p.batch), dim3(W * 64), 0, s, p);
-    if (p.parts > 1) launch_merge<DT, D, IO, wide_step_tiles(SPLIT_IO<IO>, CT)>(p, W * CT, s);
+    hipLaunchKernelGGL((tree_wide<DT, D, IO, CT, W>), dim3(p.hkv * p.col_groups, p.rows), dim3(W * 64), 0, s, p);
+    if (p.slot_rows) launch_merge<DT, D, IO>(p, W * CT, s);
 }
 
 template <int DT, int D, typename IO>

@@ -339,6 +339,8 @@ def _i32(t, device):
     """An index tensor as contiguous int32 on the pool's device (the C-ABI reads int32)."""
     import torch
 
+    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
     out = torch.as_tensor(t).to(device=device, dtype=torch.int32).contiguous()
     if out.device != torch.device(device):
         raise VspecRocmError(f"index tensor on {out.device}, the pool is on {device}")

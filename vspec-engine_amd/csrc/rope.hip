@@ -33,6 +33,15 @@ struct RopeParams {
     double turns[kMaxPairs];  // turns a position
 };
 
+// The pair turned by t = (cos, sin), alike on every path: the sums are held in f32 (left to the compiler, some calls
+// round them to f16 within the multiply-add and some after it).
+__device__ __forceinline__ float2 turned(float x1, float x2, float2 t) {
+    float y1 = fmaf(x1, t.x, -(x2 * t.y)), y2 = fmaf(x1, t.y, x2 * t.x);
+    asm("" : "+v"(y1), "+v"(y2));
+    return make_float2(y1, y2);
+}
+
+// Element by element: any alignment, strides and rope_dim.
 template <typename T>
 __global__ __launch_bounds__(256) void rope_rows(RopeParams p, bool interleaved) {
     __shared__ float2 cs[kMaxPairs];
@@ -61,8 +70,93 @@ __global__ __launch_bounds__(256) void rope_rows(RopeParams p, bool interleaved)
         const uint32_t e1 = interleaved ? 2 * u : u, e2 = interleaved ? 2 * u + 1 : u + half;
         const float x1 = (float)in[e1], x2 = (float)in[e2];
         const float2 t = cs[u];
-        out[e1] = (T)(x1 * t.x - x2 * t.y);
-        out[e2] = (T)(x1 * t.y + x2 * t.x);
+        const float2 y = turned(x1, x2, t);
+        out[e1] = (T)y.x;
+        out[e2] = (T)y.y;
+    }
+}
+
+// The same where every row is whole 16-byte chunks of V elements: a unit is the two chunks whose elements pair up (half
+// layout), the chunk that holds its pairs (interleaved), or a chunk past rope_dim, which is copied.
+struct RopeSplit {
+    uint32_t tokens;                  // of a workgroup
+    uint32_t turning, units;          // units of a row that turn, all of them
+    uint32_t half_magic, units_magic, rows_magic;  // chunk_div of rope_dim / 2, units, heads of q and k
+};
+constexpr uint32_t kChunkTokens = 4, kChunkHeads = 8192;  // (as many rows as chunk_div divides)
+
+// x / d for x below 2^32 / d, with magic = ceil(2^32 / d) (0 for d = 1): x magic is above x 2^32 / d by less than x,
+// that is, less than the 2^32 / d that the fraction leaves.
+__device__ __forceinline__ uint32_t chunk_div(uint32_t x, uint32_t magic) { return magic ? __umulhi(x, magic) : x; }
+uint32_t chunk_magic(uint32_t d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
+
+template <typename T, bool INTER>
+__global__ __launch_bounds__(256) void rope_chunks(RopeParams p, RopeSplit w) {
+    constexpr int V = 16 / sizeof(T);
+    struct __align__(16) Chunk {
+        T x[V];
+    };
+    __shared__ __align__(16) float2 cs[kChunkTokens][kMaxPairs];
+    const uint32_t token0 = blockIdx.x * w.tokens, tokens = min(w.tokens, p.tokens - token0);
+    const uint32_t half = p.rope_dim / 2;
+    for (uint32_t i = threadIdx.x; i < tokens * half; i += 256) {
+        const uint32_t at = chunk_div(i, w.half_magic), u = i - at * half;
+        const double t = (double)p.positions[token0 + at] * p.turns[u];
+        float s, c;
+        sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+        cs[at][u] = make_float2(p.magnitude * c, p.sign * p.magnitude * s);
+    }
+    __syncthreads();
+    const uint32_t rows = p.q.heads + p.k.heads, all = tokens * rows * w.units;
+    constexpr int kBatch = 4;  // units of a thread whose loads are on their way
+    for (uint32_t base = threadIdx.x; base < all; base += 256 * kBatch) {
+        Chunk a[kBatch], b[INTER ? 1 : kBatch];
+        T* out[kBatch];
+        uint32_t at[kBatch], unit[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const uint32_t idx = min(base + 256 * i, all - 1);
+            const uint32_t r = chunk_div(idx, w.units_magic), u = idx - r * w.units;
+            at[i] = chunk_div(r, w.rows_magic);
+            unit[i] = u;
+            uint32_t h = r - at[i] * rows;
+            const bool isk = h >= p.q.heads;
+            h -= isk ? p.q.heads : 0u;
+            const RopeOperand& o = isk ? p.k : p.q;
+            const int64_t token = token0 + at[i];
+            const uint32_t e = u < w.turning ? V * u : p.rope_dim + V * (u - w.turning);
+            const T* in = reinterpret_cast<const T*>(o.in) + token * o.in_token + (int64_t)h * o.in_head + e;
+            out[i] = reinterpret_cast<T*>(o.out) + token * o.out_token + (int64_t)h * o.out_head + e;
+            a[i] = *reinterpret_cast<const Chunk*>(in);
+            if constexpr (!INTER) b[i] = u < w.turning ? *reinterpret_cast<const Chunk*>(in + half) : a[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (base + 256 * i >= all) continue;
+            if (unit[i] < w.turning) {
+                if constexpr (INTER) {
+                    const float2* t = cs[at[i]] + V / 2 * unit[i];
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        const float x1 = (float)a[i].x[e], x2 = (float)a[i].x[e + 1];
+                        const float2 y = turned(x1, x2, t[e / 2]);
+                        a[i].x[e] = (T)y.x;
+                        a[i].x[e + 1] = (T)y.y;
+                    }
+                } else {
+                    const float2* t = cs[at[i]] + V * unit[i];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float x1 = (float)a[i].x[e], x2 = (float)b[i].x[e];
+                        const float2 y = turned(x1, x2, t[e]);
+                        a[i].x[e] = (T)y.x;
+                        b[i].x[e] = (T)y.y;
+                    }
+                    *reinterpret_cast<Chunk*>(out[i] + half) = b[i];
+                }
+            }
+            *reinterpret_cast<Chunk*>(out[i]) = a[i];
+        }
     }
 }
 
@@ -136,6 +230,12 @@ int rope_operand(const VspecRopeRows* r, const VspecRopeDesc* d, const char* whi
     return 1;
 }
 
+// Whether an operand's rows start at whole 16-byte chunks of v elements.
+bool whole_chunks(const RopeOperand& o, uint32_t v) {
+    return o.heads == 0 || ((((uintptr_t)o.in | (uintptr_t)o.out) % 16) == 0 &&
+                            ((o.in_token | o.in_head | o.out_token | o.out_head) & (int64_t)(v - 1)) == 0);
+}
+
 }  // namespace
 }  // namespace vkv
 
@@ -176,9 +276,26 @@ extern "C" int vspec_rocm_rope(const VspecRopeDesc* d) {
     p.head_dim = d->head_dim;
     p.rope_dim = d->rope_dim;
     p.sign = d->inverse ? -1.0f : 1.0f;
-    const bool inter = d->layout == VSPEC_ROPE_INTERLEAVED;
+    const bool inter = d->layout == VSPEC_ROPE_INTERLEAVED, f32 = d->dtype == VSPEC_KV_F32;
     hipStream_t s = (hipStream_t)d->stream;
-    if (d->dtype == VSPEC_KV_F32) {
+    // By chunks where rows, strides and the turned part are whole ones (16384 tokens of 40 heads: 215 us by
+    // elements, TIMED by chunks).  Tokens share a workgroup where that still leaves 4 to a CU.
+    const uint32_t v = f32 ? 4 : 8, turned = inter ? d->rope_dim : d->rope_dim / 2;
+    if (heads <= kChunkHeads && d->head_dim % v == 0 && turned % v == 0 && whole_chunks(p.q, v) && whole_chunks(p.k, v)) {
+        RopeSplit w = {};
+        w.tokens = kChunkTokens;
+        while (w.tokens > 1 && d->num_tokens / w.tokens < 4u * host_num_cus()) w.tokens /= 2;
+        w.turning = turned / v;
+        w.units = w.turning + (d->head_dim - d->rope_dim) / v;
+        w.half_magic = chunk_magic(d->rope_dim / 2);
+        w.units_magic = chunk_magic(w.units);
+        w.rows_magic = chunk_magic((uint32_t)heads);
+        const dim3 grid((p.tokens + w.tokens - 1) / w.tokens);
+        if (f32 && inter) hipLaunchKernelGGL((rope_chunks<float, true>), grid, dim3(256), 0, s, p, w);
+        else if (f32) hipLaunchKernelGGL((rope_chunks<float, false>), grid, dim3(256), 0, s, p, w);
+        else if (inter) hipLaunchKernelGGL((rope_chunks<_Float16, true>), grid, dim3(256), 0, s, p, w);
+        else hipLaunchKernelGGL((rope_chunks<_Float16, false>), grid, dim3(256), 0, s, p, w);
+    } else if (f32) {
         hipLaunchKernelGGL((rope_rows<float>), dim3(p.tokens), dim3(256), 0, s, p, inter);
     } else {
         hipLaunchKernelGGL((rope_rows<_Float16>), dim3(p.tokens), dim3(256), 0, s, p, inter);

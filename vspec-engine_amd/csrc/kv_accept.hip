@@ -2,17 +2,29 @@
 // between slots of one sequence, in the pools of all layers.
 //
 // Sources and destinations of a sequence overlap, so every row is read before any is written.
-// Rows move unit by unit: a unit is a column of all rows (16 bytes of K, of V in f32 pools; the
-// scattered elements of V in f16 and int4 tiles, kv_common.h; one scale), and units are
-// independent of each other.  A workgroup holds one (layer, sequence, kv head) and K or V; its
-// threads take (row, unit) pairs, kBatch of them in registers between two barriers.
+// Rows move column by column, a column being 16 bytes of every row, and columns are independent
+// of each other:
+//   K, and V of f32 pools       16 bytes of a token's row
+//   V of f16 and int4 pools     16 bytes of a group of 4 tokens, which hold a part of each
+//                               (kv_common.h): a destination group is put together from the up to
+//                               four groups that its tokens come from and written whole (by
+//                               single bytes, 64 x 64 nodes in 16 int4 layers took 71 us)
+// A workgroup, one wave, holds one (sequence, kv head) and K or V of some layers; what a row's slots
+// are is worked out once for them.  It takes a pass of columns into registers and writes them.
+//
+// The bytes are few (64 x 64 nodes, 16 int4 layers: 26 MB, 5 us at the rate of a large copy); what
+// counts is the chain of waits, path -> table -> row -> write, and how many of them overlap.  So
+// workgroups are small and take only as many layers as leave 24 of them to a CU (four waves and
+// 8 layers a workgroup: 37 us; this: TIMED).
+#include <type_traits>
+
 #include "host.h"
 #include "kv_common.h"
 
 namespace vkv {
 namespace {
 
-constexpr uint32_t kLayers = 32;  // pools of one launch: their addresses are kernel arguments
+constexpr uint32_t kLayers = 64;  // pools of one launch: their addresses are kernel arguments
 constexpr uint32_t kNodes = 64;
 
 struct AcceptPool {
@@ -31,114 +43,168 @@ struct AcceptParams {
     int32_t* new_lens;  // or null
     uint32_t max_blocks, max_path, num_nodes;
     uint32_t hkv, head_dim, block_tokens, num_blocks;
+    uint32_t layers, share;  // pools of this launch, and of a workgroup
 };
 
-// Where slot `pos` of sequence b lies: its (block, head) index and the slot in the block.
-__device__ __forceinline__ bool accept_slot(const AcceptParams& p, uint32_t b, int64_t pos, uint32_t h, size_t* bh,
-                                            uint32_t* slot) {
-    if (pos < 0 || pos >= (int64_t)p.max_blocks * p.block_tokens) return false;
-    const int entry = p.block_tables[(size_t)b * p.max_blocks + (uint32_t)(pos / p.block_tokens)];
+// Where slot `pos` of sequence b lies for kv head h: the index of its token, and its slot in the block.
+__device__ __forceinline__ bool accept_slot(const AcceptParams& p, uint32_t b, uint32_t pos, uint32_t h, size_t* token, uint32_t* slot) {
+    const uint32_t row = pos / p.block_tokens;
+    if (row >= p.max_blocks) return false;
+    const int entry = p.block_tables[(size_t)b * p.max_blocks + row];
     if (entry < 0 || (uint32_t)entry >= p.num_blocks) return false;
-    *bh = (size_t)entry * p.hkv + h;
-    *slot = (uint32_t)(pos % p.block_tokens);
+    *slot = pos - row * p.block_tokens;
+    *token = ((size_t)entry * p.hkv + h) * p.block_tokens + *slot;
     return true;
 }
 
+// 16 bytes of V of a group of 4 tokens: the bits of token r.
 template <int DT>
-__global__ __launch_bounds__(256) void kv_accept(AcceptParams p) {
+__device__ __forceinline__ uint64_t token_bits(uint64_t w, uint32_t r) {
+    if constexpr (DT == VSPEC_KV_F16) return (w >> (16 * r)) & 0xffffull;
+    return (w >> (8 * (2 * (r & 1) + (r >> 1)))) & 0x000000ff000000ffull;
+}
+template <int DT>
+__device__ __forceinline__ uint64_t bits_of_token(uint64_t x, uint32_t r) {
+    if constexpr (DT == VSPEC_KV_F16) return x << (16 * r);
+    return x << (8 * (2 * (r & 1) + (r >> 1)));
+}
+
+template <int DT>
+__global__ __launch_bounds__(64) void kv_accept(AcceptParams p) {
+    constexpr uint32_t kThreads = 64;
     const uint32_t h = blockIdx.x, b = blockIdx.y;
     const bool isv = blockIdx.z & 1u;
-    const AcceptPool& pool = p.pools[blockIdx.z >> 1];
-    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t lane = threadIdx.x;
     // the path's length: lanes before the first entry that names no node
     const int32_t node_l = lane < p.max_path ? p.path[(size_t)b * p.max_path + lane] : -1;
     const uint64_t ends = __builtin_amdgcn_ballot_w64(node_l < 0 || (uint32_t)node_l >= p.num_nodes);
     const uint32_t count = ends ? (uint32_t)__builtin_ctzll(ends) : 64u;
-    const int64_t start = max(p.start_pos[b], 0);
-    if (h == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.new_lens) p.new_lens[b] = (int32_t)(start + count);
+    const uint32_t start = (uint32_t)max(p.start_pos[b], 0);
+    if (h == 0 && blockIdx.z == 0 && lane == 0 && p.new_lens) p.new_lens[b] = (int32_t)(start + count);
 
     // row `lane` of the path
-    __shared__ size_t from_bh[kNodes], to_bh[kNodes];
-    __shared__ uint32_t from_slot[kNodes], to_slot[kNodes];
-    __shared__ bool moves[kNodes];
-    if (threadIdx.x < 64) {
-        size_t fb = 0, tb = 0;
-        uint32_t fs = 0, ts = 0;
-        bool ok = lane < count && node_l != (int32_t)lane;
-        ok = ok && accept_slot(p, b, start + node_l, h, &fb, &fs);
-        ok = ok && accept_slot(p, b, start + lane, h, &tb, &ts);
-        from_bh[lane] = fb;
-        to_bh[lane] = tb;
-        from_slot[lane] = fs;
-        to_slot[lane] = ts;
-        moves[lane] = ok;
-    }
+    __shared__ size_t from_sh[kNodes], to_sh[kNodes];
+    size_t from = 0, to = 0;
+    uint32_t fs = 0, ts = 0;
+    bool ok = lane < count && node_l != (int32_t)lane;
+    ok = ok && accept_slot(p, b, start + node_l, h, &from, &fs);
+    ok = ok && accept_slot(p, b, start + lane, h, &to, &ts);
+    from_sh[lane] = from;
+    to_sh[lane] = to;
+    const uint64_t moves = __builtin_amdgcn_ballot_w64(ok);
+    if (moves == 0) return;
     __syncthreads();
     const uint32_t D = p.head_dim, P = p.block_tokens, G = D / 32;
+    const uint32_t rb = DT == VSPEC_KV_F32 ? 4 * D : DT == VSPEC_KV_F16 ? 2 * D : D / 2;  // bytes of a row
+    const uint32_t first = (blockIdx.z >> 1) * p.share, last = min(first + p.share, p.layers);
 
-    // unit u of a row: read(bh, slot, u) and write(bh, slot, u, x)
-    auto move = [&](const uint32_t units, auto read, auto write) {
-        typedef decltype(read((size_t)0, 0u, 0u)) T;
-        constexpr int kBatch = 4;
-        const uint32_t wide = (256u / kNodes) * kBatch;  // units between two barriers
-        const uint32_t row = threadIdx.x % kNodes, u0 = threadIdx.x / kNodes;
-        const bool mine = moves[row];
-        for (uint32_t base = 0; base < units; base += wide) {
-            T x[kBatch];
+    // x / d, d <= 4096 and x below 2^20: magic is above 2^32 / d by less than 1
+    auto magic_of = [](const uint32_t d) -> uint32_t { return d == 1 ? 0u : 0xffffffffu / d + 1u; };
+    auto div = [](const uint32_t x, const uint32_t magic) -> uint32_t { return magic ? __umulhi(x, magic) : x; };
+    auto moved = [&](const uint32_t row) -> bool { return row < 64u && (moves >> row) & 1u; };
+
+    // columns of `rows` things, read(row, column) and write(row, column, x): up to N a thread and pass
+    auto pass = [&](auto batch, const uint32_t rows, const uint32_t columns, auto wanted, auto read, auto write) {
+        constexpr int N = decltype(batch)::value;
+        typedef decltype(read(0u, 0u)) T;
+        const uint32_t most = N * kThreads / rows;
+        for (uint32_t c0 = 0; c0 < columns; c0 += most) {
+            const uint32_t n = min(most, columns - c0), magic = magic_of(n);
+            T x[N];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const uint32_t u = base + u0 + i * (256u / kNodes);
-                if (mine && u < units) x[i] = read(from_bh[row], from_slot[row], u);
+            for (int i = 0; i < N; ++i) {
+                const uint32_t idx = threadIdx.x + kThreads * i, row = div(idx, magic);
+                if (row < rows && wanted(row)) x[i] = read(row, c0 + idx - row * n);
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const uint32_t u = base + u0 + i * (256u / kNodes);
-                if (mine && u < units) write(to_bh[row], to_slot[row], u, x[i]);
+            for (int i = 0; i < N; ++i) {
+                const uint32_t idx = threadIdx.x + kThreads * i, row = div(idx, magic);
+                if (row < rows && wanted(row)) write(row, c0 + idx - row * n, x[i]);
             }
         }
     };
 
-    if constexpr (DT == VSPEC_KV_INT4) {
-        if (!isv) {
-            const uint32_t rb = D / 2;
-            move(rb / 16, [&](size_t bh, uint32_t s, uint32_t u) { return reinterpret_cast<const uint4*>(pool.k + (bh * P + s) * rb)[u]; },
-                 [&](size_t bh, uint32_t s, uint32_t u, uint4 x) { reinterpret_cast<uint4*>(pool.k + (bh * P + s) * rb)[u] = x; });
-            move(G, [&](size_t bh, uint32_t s, uint32_t u) { return pool.ks[int4_ks_index(bh, G, P, s, u)]; },
-                 [&](size_t bh, uint32_t s, uint32_t u, uint16_t x) { pool.ks[int4_ks_index(bh, G, P, s, u)] = x; });
-            if (pool.kf) {
-                // one bit a row: words are shared between rows, and no other workgroup's
-                auto word = [&](size_t bh, uint32_t s) { return pool.kf + bh * (P / 16) + s / 16; };
-                uint32_t bit = 0;
-                const bool mine = threadIdx.x < 64 && moves[lane];
-                if (mine) bit = *word(from_bh[lane], from_slot[lane]) >> (from_slot[lane] % 16) & 1u;
-                __syncthreads();
-                if (mine) {
-                    const uint32_t m = 1u << (to_slot[lane] % 16);
-                    if (bit) atomicOr(word(to_bh[lane], to_slot[lane]), m);
-                    else atomicAnd(word(to_bh[lane], to_slot[lane]), ~m);
-                }
+    if (DT != VSPEC_KV_F32 && isv) {
+        const uint32_t group0 = start / 4, groups = (start + count - 1) / 4 - group0 + 1;  // P is a multiple of 16
+        // rows of the path in group i, as bits: token r is row 4 (group0 + i) + r - start
+        auto rows_in = [&](const uint32_t i) -> uint32_t {
+            const int at = (int)(4 * (group0 + i)) - (int)start;
+            return (uint32_t)(at < 0 ? moves << -at : at < 64 ? moves >> at : 0) & 15u;
+        };
+        for (uint32_t l = first; l < last; ++l) {
+            const AcceptPool& pool = p.pools[l];
+            uint16_t scale[4] = {0, 0, 0, 0};  // of row `lane`
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {
+                if (DT == VSPEC_KV_INT4 && ok && c < G) scale[c] = pool.vs[from * G + c];
             }
-        } else {
-            // byte u: a token's codes of two elements
-            auto at = [&](size_t bh, uint32_t s, uint32_t u) {
-                uint32_t high;
-                return pool.v + int4_v_byte(bh, P, D, s, 32u * (u / 16) + u % 16, &high);
-            };
-            move(D / 2, [&](size_t bh, uint32_t s, uint32_t u) { return *at(bh, s, u); },
-                 [&](size_t bh, uint32_t s, uint32_t u, uint8_t x) { *at(bh, s, u) = x; });
-            move(G, [&](size_t bh, uint32_t s, uint32_t u) { return pool.vs[(bh * P + s) * G + u]; },
-                 [&](size_t bh, uint32_t s, uint32_t u, uint16_t x) { pool.vs[(bh * P + s) * G + u] = x; });
+            pass(std::integral_constant<int, 5>(), groups, rb / 4, [&](uint32_t i) { return rows_in(i) != 0; },
+                 [&](uint32_t i, uint32_t u) {
+                     const uint32_t in = rows_in(i);
+                     const uint32_t any = __builtin_ctz(in), row0 = 4 * (group0 + i) - start;  // (row0 + r wraps back for r in `in`)
+                     const size_t own = to_sh[row0 + any] - any;
+                     uint4 w[4];
+                     uint32_t r_of[4];
+#pragma unroll
+                     for (uint32_t r = 0; r < 4; ++r) {
+                         const size_t from = (in >> r) & 1u ? from_sh[row0 + r] : own + r;
+                         r_of[r] = (uint32_t)from & 3u;
+                         w[r] = reinterpret_cast<const uint4*>(pool.v + (from - r_of[r]) * rb)[u];
+                     }
+                     uint64_t lo = 0, hi = 0;
+#pragma unroll
+                     for (uint32_t r = 0; r < 4; ++r) {
+                         lo |= bits_of_token<DT>(token_bits<DT>((uint64_t)w[r].y << 32 | w[r].x, r_of[r]), r);
+                         hi |= bits_of_token<DT>(token_bits<DT>((uint64_t)w[r].w << 32 | w[r].z, r_of[r]), r);
+                     }
+                     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+                 },
+                 [&](uint32_t i, uint32_t u, uint4 x) {
+                     const uint32_t any = __builtin_ctz(rows_in(i)), row0 = 4 * (group0 + i) - start;
+                     reinterpret_cast<uint4*>(pool.v + (to_sh[row0 + any] - any) * rb)[u] = x;
+                 });
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {
+                if (DT == VSPEC_KV_INT4 && ok && c < G) pool.vs[to * G + c] = scale[c];
+            }
+            for (uint32_t c = 4; DT == VSPEC_KV_INT4 && c < G; ++c) {
+                if (ok) scale[0] = pool.vs[from * G + c];
+                __syncthreads();
+                if (ok) pool.vs[to * G + c] = scale[0];
+            }
         }
-    } else if (DT == VSPEC_KV_F16 && isv) {
-        uint16_t* v = reinterpret_cast<uint16_t*>(pool.v);
-        move(D, [&](size_t bh, uint32_t s, uint32_t u) { return v[f16_v_index(bh, P, D, s, u)]; },
-             [&](size_t bh, uint32_t s, uint32_t u, uint16_t x) { v[f16_v_index(bh, P, D, s, u)] = x; });
-    } else {
-        const uint32_t rb = D * (DT == VSPEC_KV_F32 ? 4u : 2u);
-        uint8_t* base = isv ? pool.v : pool.k;
-        move(rb / 16, [&](size_t bh, uint32_t s, uint32_t u) { return reinterpret_cast<const uint4*>(base + (bh * P + s) * rb)[u]; },
-             [&](size_t bh, uint32_t s, uint32_t u, uint4 x) { reinterpret_cast<uint4*>(base + (bh * P + s) * rb)[u] = x; });
+        return;
+    }
+    for (uint32_t l = first; l < last; ++l) {
+        const AcceptPool& pool = p.pools[l];
+        uint8_t* const base = isv ? pool.v : pool.k;
+        uint16_t scale[4] = {0, 0, 0, 0};  // of row `lane`, and its flag
+        uint32_t flag = 0;
+        auto scale_at = [&](const size_t token, const uint32_t slot, const uint32_t c) { return pool.ks + (token - slot) * G + (size_t)c * P + slot; };
+        auto flag_at = [&](const size_t token) { return pool.kf + token / 16; };  // a bit a row, in words of 16
+        const bool scales = DT == VSPEC_KV_INT4 && ok;
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            if (scales && c < G) scale[c] = *scale_at(from, fs, c);
+        }
+        if (scales && pool.kf) flag = (*flag_at(from) >> (fs % 16)) & 1u;
+        pass(std::integral_constant<int, 8>(), count, rb / 16, moved, [&](uint32_t row, uint32_t u) { return reinterpret_cast<const uint4*>(base + from_sh[row] * rb)[u]; },
+             [&](uint32_t row, uint32_t u, uint4 x) { reinterpret_cast<uint4*>(base + to_sh[row] * rb)[u] = x; });
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            if (scales && c < G) *scale_at(to, ts, c) = scale[c];
+        }
+        if (scales && pool.kf) {
+            const uint32_t m = 1u << (ts % 16);
+            if (flag) atomicOr(flag_at(to), m);
+            else atomicAnd(flag_at(to), ~m);
+        }
+        for (uint32_t c = 4; DT == VSPEC_KV_INT4 && c < G; ++c) {
+            if (ok) scale[0] = *scale_at(from, fs, c);
+            __syncthreads();
+            if (ok) *scale_at(to, ts, c) = scale[0];
+        }
     }
 }
 
@@ -206,11 +272,14 @@ extern "C" int vspec_rocm_kv_accept(const VspecPagedKV* kvs, uint32_t num_kvs, u
                           kv.dtype == VSPEC_KV_INT4 ? kv.k_flags : nullptr};
         }
         p.new_lens = at == 0 ? new_lens : nullptr;
-        const dim3 grid(p.hkv, batch, 2 * n);
+        p.layers = n;
+        const uint64_t all = 2ull * n * p.hkv * batch, target = 24ull * host_num_cus();
+        p.share = (uint32_t)(all <= target ? 1 : (all + target - 1) / target < n ? (all + target - 1) / target : n);
+        const dim3 grid(p.hkv, batch, 2 * ((n + p.share - 1) / p.share));
         switch (kvs[0].dtype) {
-            case VSPEC_KV_F32: hipLaunchKernelGGL((kv_accept<VSPEC_KV_F32>), grid, dim3(256), 0, s, p); break;
-            case VSPEC_KV_F16: hipLaunchKernelGGL((kv_accept<VSPEC_KV_F16>), grid, dim3(256), 0, s, p); break;
-            default: hipLaunchKernelGGL((kv_accept<VSPEC_KV_INT4>), grid, dim3(256), 0, s, p); break;
+            case VSPEC_KV_F32: hipLaunchKernelGGL((kv_accept<VSPEC_KV_F32>), grid, dim3(64), 0, s, p); break;
+            case VSPEC_KV_F16: hipLaunchKernelGGL((kv_accept<VSPEC_KV_F16>), grid, dim3(64), 0, s, p); break;
+            default: hipLaunchKernelGGL((kv_accept<VSPEC_KV_INT4>), grid, dim3(64), 0, s, p); break;
         }
     }
     const hipError_t e = hipGetLastError();

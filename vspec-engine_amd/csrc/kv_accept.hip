@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64) void kv_accept(AcceptParams p) {
     auto div = [](const uint32_t x, const uint32_t magic) -> uint32_t { return magic ? __umulhi(x, magic) : x; };
     auto moved = [&](const uint32_t row) -> bool { return row < 64u && (moves >> row) & 1u; };
 
-    // columns of `rows` things, read(row, column) and write(row, column, x): up to N a thread and pass
+    // columns of `rows` things, read(row, column) and, if wanted(row), write(row, column, x): up to N a thread and pass
     auto pass = [&](auto batch, const uint32_t rows, const uint32_t columns, auto wanted, auto read, auto write) {
         constexpr int N = decltype(batch)::value;
         typedef decltype(read(0u, 0u)) T;
@@ -113,13 +113,14 @@ __global__ __launch_bounds__(64) void kv_accept(AcceptParams p) {
             T x[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const uint32_t idx = threadIdx.x + kThreads * i, row = div(idx, magic);
-                if (row < rows && wanted(row)) x[i] = read(row, c0 + idx - row * n);
+                // (every lane reads, so that no load waits for the one before it)
+                const uint32_t idx = min(lane + kThreads * i, rows * n - 1), row = div(idx, magic);
+                if (kThreads * i < rows * n) x[i] = read(row, c0 + idx - row * n);
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const uint32_t idx = threadIdx.x + kThreads * i, row = div(idx, magic);
+                const uint32_t idx = lane + kThreads * i, row = div(idx, magic);
                 if (row < rows && wanted(row)) write(row, c0 + idx - row * n, x[i]);
             }
         }
@@ -142,8 +143,8 @@ __global__ __launch_bounds__(64) void kv_accept(AcceptParams p) {
             pass(std::integral_constant<int, 5>(), groups, rb / 4, [&](uint32_t i) { return rows_in(i) != 0; },
                  [&](uint32_t i, uint32_t u) {
                      const uint32_t in = rows_in(i);
-                     const uint32_t any = __builtin_ctz(in), row0 = 4 * (group0 + i) - start;  // (row0 + r wraps back for r in `in`)
-                     const size_t own = to_sh[row0 + any] - any;
+                     const uint32_t any = __builtin_ctz(in | 16u), row0 = 4 * (group0 + i) - start;  // (row0 + r wraps back for r in `in`)
+                     const size_t own = in ? to_sh[row0 + any] - any : 0;
                      uint4 w[4];
                      uint32_t r_of[4];
 #pragma unroll

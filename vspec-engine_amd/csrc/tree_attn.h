@@ -215,9 +215,14 @@ __device__ __forceinline__ TreeJob tree_job(const TreeParams& p, int row, int un
 template <typename T>
 __device__ __forceinline__ T own_scalar(T x) {
     T y;
-    if constexpr (sizeof(T) == 8) asm volatile("s_mov_b64 %0, %1" : "=s"(y) : "s"(x));
-    else asm volatile("s_mov_b32 %0, %1" : "=s"(y) : "s"(x));
+    asm volatile("s_mov_b32 %0, %1" : "=s"(y) : "s"(x));
     return y;
+}
+template <typename T>
+__device__ __forceinline__ T* own_scalar(T* x) {
+    uint64_t y;
+    asm volatile("s_mov_b64 %0, %1" : "=s"(y) : "s"(x));
+    return (T*)(__attribute__((address_space(1))) T*)y;  // (device memory: a pointer of unknown origin is read by flat loads, which also wait for LDS)
 }
 
 // The kernel's own arguments, read again where they are needed: kept from the start they would fill the scalar

@@ -252,7 +252,7 @@ constexpr int tree_step_tiles(int dtype) { return dtype == VSPEC_KV_F32 ? 1 : 2;
 // Workgroups of tree_mfma.hip that a CU holds.  Two hide each other's waits, where 256 registers a
 // lane hold K, V, q and the output without spilling more than a few.
 constexpr int tree_cu_groups(int dtype, int d, bool f32_rows, int ct) {
-    return ct == 1 || d == 64 || dtype == VSPEC_KV_F32 || (dtype == VSPEC_KV_F16 && !f32_rows) ? 2 : 1;
+    return ct == 1 || d == 64 || dtype == VSPEC_KV_F32 || !f32_rows ? 2 : 1;
 }
 
 }  // namespace vkv

@@ -60,8 +60,8 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
     constexpr int NDT = D / 16;  // d-tiles of the output
     typedef Tile<DT, D> T;
     __shared__ uint64_t bits_sh[64];
-    __shared__ f4_t red[4][NDT][64];
-    __shared__ float red_ml[4][16][2];
+    __shared__ f4_t red[CT][4][NDT][64];
+    __shared__ float red_ml[CT][4][16][2];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -78,7 +78,29 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
     const int lo = job.lo, hi = job.hi;
 
     if (threadIdx.x < p.nodes) bits_sh[threadIdx.x] = tree_bits(p, b, threadIdx.x, sp.len);
-    __syncthreads();
+
+    // ---- q: columns of this wave, on their way before K and V (loads come back in order) ----
+    // Column c is node c / group, head c % group of the kv head's.
+    const int cols = (int)(p.nodes * p.group);
+    const int ctile0 = ((int)cg * (int)p.col_waves + cw) * CT;
+    typedef IO raw_t __attribute__((ext_vector_type(4)));
+    raw_t raw[CT][D / 16];
+    bool live[CT];
+    int node[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int c = (ctile0 + ct) * 16 + n;
+        const int i = c / (int)p.group;
+        node[ct] = min(i, (int)p.nodes - 1);
+        live[ct] = c < cols && i < sp.len;
+        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live[ct] ? i : 0)) * p.hq + (size_t)h * p.group + (live[ct] ? c - i * (int)p.group : 0)) * D;
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+            // four adjacent elements: of the lane's 8 of k-step u / 2 (f16: 32i + 8g, int4: 8 (g NQ + i)), or f32's 16u + 4g
+            const int d = F32 ? 16 * u + 4 * g : (DT == VSPEC_KV_F16 ? 32 * (u / 2) + 8 * g : 8 * (g * NQ + u / 2)) + 4 * (u % 2);
+            raw[ct][u] = *reinterpret_cast<const raw_t*>(src + d);
+        }
+    }
 
     const int P = (int)own_scalar(p.block_tokens);
     const int32_t* const tables = own_scalar(p.block_tables + (size_t)b * p.max_blocks);
@@ -197,42 +219,21 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
         load_v(now.token[a], tile[a]);
     }
 
-    // ---- q: columns of this wave ----
-    // Column c is node c / group, head c % group of the kv head's.  The operands hold clip(q) 2^e
-    // (e != 0 only for f32 rows outside f16's range, qnorm_shift); scores come out in that unit
-    // and fac takes them to log2 units.
-    const int cols = (int)(p.nodes * p.group);
-    const int ctile0 = ((int)cg * (int)p.col_waves + cw) * CT;
+    // The operands of q hold clip(q) 2^e (e != 0 only for f32 rows outside f16's range,
+    // qnorm_shift); scores come out in that unit and fac takes them to log2 units.
     h8_t qh[F32 ? 1 : CT][NQ], ql[SPLIT ? CT : 1][NQ];
     float qf[F32 ? CT : 1][F32 ? D / 4 : 1];
     float fac[CT];
-    int node[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        const int c = (ctile0 + ct) * 16 + n;
-        const int i = c / (int)p.group;
-        node[ct] = min(i, (int)p.nodes - 1);
-        const bool live = c < cols && i < sp.len;
-        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live ? i : 0)) * p.hq + (size_t)h * p.group + (live ? c - i * (int)p.group : 0)) * D;
         constexpr int E = D / 4;
         float x[E];
 #pragma unroll
-        for (int u = 0; u < E / 4; ++u) {
-            // four adjacent elements: of the lane's 8 of k-step u / 2 (f16: 32i + 8g, int4: 8 (g NQ + i)), or f32's 16u + 4g
-            const int d = F32 ? 16 * u + 4 * g : (DT == VSPEC_KV_F16 ? 32 * (u / 2) + 8 * g : 8 * (g * NQ + u / 2)) + 4 * (u % 2);
-            if constexpr (sizeof(IO) == 4) {
-                const float4 w = *reinterpret_cast<const float4*>(src + d);
-                x[4 * u] = w.x, x[4 * u + 1] = w.y, x[4 * u + 2] = w.z, x[4 * u + 3] = w.w;
-            } else {
-                const h4_t w = *reinterpret_cast<const h4_t*>(src + d);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * u + e] = (float)w[e];
-            }
-        }
+        for (int e = 0; e < E; ++e) x[e] = (float)raw[ct][e / 4][e % 4];
         float sum = 0.f, var = 0.f, am = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[e] = live ? x[e] : 0.f;
+            x[e] = live[ct] ? x[e] : 0.f;
             sum += x[e];
         }
         sum = add_rows(sum);
@@ -291,6 +292,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
         return seen & (left >= 4 ? 15u : left > 0 ? (1u << left) - 1u : 0u);
     };
     bool wild = false;  // V held what is not finite, among nodes
+    __syncthreads();    // (bits_sh)
 
     // K's registers take the next step's as soon as the scores are there, V's at the end.
     auto process = [&](const int step, const Where& s, const Where& next) {
@@ -707,35 +709,40 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
 #pragma unroll
         for (int r = 0; r < 4; ++r) dst[out_dim<DT>(j, g, r)] = (IO)(empty ? 0.f : a[r] / sum);
     };
+    float sum[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) sum[ct] = add_rows(l[ct]);
+    if (token_waves == 1) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int j = 0; j < NDT; ++j) finish(ct, j, acc[ct][j], sum[ct], mf[ct]);
+        }
+        return;
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        const float sum = add_rows(l[ct]);
-        if (token_waves == 1) {
-#pragma unroll
-            for (int j = 0; j < NDT; ++j) finish(ct, j, acc[ct][j], sum, mf[ct]);
-            continue;
-        }
-        if (ct) __syncthreads();
         if (g == 0) {
-            red_ml[wave][n][0] = mf[ct];
-            red_ml[wave][n][1] = sum;
+            red_ml[ct][wave][n][0] = mf[ct];
+            red_ml[ct][wave][n][1] = sum[ct];
         }
-        __syncthreads();
-        float top = -INFINITY, total = 0.f;
-        for (int t = 0; t < token_waves; ++t) top = fmaxf(top, red_ml[cw * token_waves + t][n][0]);
-        for (int t = 0; t < token_waves; ++t) {
-            const float* ml = red_ml[cw * token_waves + t][n];
-            total += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top);
-        }
-        const float f = __builtin_amdgcn_exp2f(mf[ct] - top);
 #pragma unroll
-        for (int j = 0; j < NDT; ++j) red[wave][j][lane] = acc[ct][j] * f;
-        __syncthreads();
-        for (int j = tw; j < NDT; j += token_waves) {
-            f4_t a = {0.f, 0.f, 0.f, 0.f};
-            for (int t = 0; t < token_waves; ++t) a += red[cw * token_waves + t][j][lane];
-            finish(ct, j, a, total, top);
+        for (int j = 0; j < NDT; ++j) red[ct][wave][j][lane] = acc[ct][j];
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int k = tw; k < CT * NDT; k += token_waves) {
+        const int ct = k / NDT, j = k - ct * NDT;
+        float top = -INFINITY, total = 0.f;
+        f4_t a = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < token_waves; ++t) top = fmaxf(top, red_ml[ct][cw * token_waves + t][n][0]);
+        for (int t = 0; t < token_waves; ++t) {
+            const float* ml = red_ml[ct][cw * token_waves + t][n];
+            const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+            total = fmaf(ml[1], f, total);
+            a += red[ct][cw * token_waves + t][j][lane] * f;
         }
+        finish(ct, j, a, total, top);
     }
 }
 

@@ -79,6 +79,24 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     const int lo = job.lo, hi = job.hi;
     if (threadIdx.x < 64) bits_sh[threadIdx.x] = threadIdx.x < p.nodes ? tree_bits(p, b, threadIdx.x, sp.len) : 0;
 
+    // q: columns of this wave, on their way before K and V (loads come back in order)
+    const int cols = (int)(p.nodes * p.group);
+    const int ctile0 = ((int)cg * W + wave) * CT;
+    typedef IO raw_t __attribute__((ext_vector_type(8), aligned(16)));
+    raw_t rawq[CT][NQ];
+    bool live[CT];
+    int node[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int c = (ctile0 + ct) * 16 + n;
+        const int i = c / (int)p.group;
+        node[ct] = min(i, (int)p.nodes - 1);
+        live[ct] = c < cols && i < sp.len;
+        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live[ct] ? i : 0)) * p.hq + (size_t)h * p.group + (live[ct] ? c - i * (int)p.group : 0)) * D;
+#pragma unroll
+        for (int k = 0; k < NQ; ++k) rawq[ct][k] = *reinterpret_cast<const raw_t*>(src + 32 * k + 8 * g);
+    }
+
     const int P = (int)own_scalar(p.block_tokens);
     const int32_t* const tables = own_scalar(p.block_tables + (size_t)b * p.max_blocks);
     const int32_t* const used = own_scalar(p.block_used ? p.block_used + (size_t)b * p.max_blocks : nullptr);
@@ -401,34 +419,14 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) held[s] = load_step(lo + s, s);
 
-    const int cols = (int)(p.nodes * p.group);
-    const int ctile0 = ((int)cg * W + wave) * CT;
     h8_t qh[CT][NQ], ql[SPLIT ? CT : 1][NQ];
     float fac[CT];
-    int node[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        const int c = (ctile0 + ct) * 16 + n;
-        const int i = c / (int)p.group;
-        node[ct] = min(i, (int)p.nodes - 1);
-        const bool live = c < cols && i < sp.len;
-        const IO* src = reinterpret_cast<const IO*>(p.q) + (((size_t)b * p.nodes + (live ? i : 0)) * p.hq + (size_t)h * p.group + (live ? c - i * (int)p.group : 0)) * D;
         float x[8 * NQ], sum = 0.f, var = 0.f, am = 0.f;
 #pragma unroll
-        for (int k = 0; k < NQ; ++k) {
-            if constexpr (SPLIT) {
-                const float4 w0 = *reinterpret_cast<const float4*>(src + 32 * k + 8 * g), w1 = *reinterpret_cast<const float4*>(src + 32 * k + 8 * g + 4);
-                x[8 * k] = w0.x, x[8 * k + 1] = w0.y, x[8 * k + 2] = w0.z, x[8 * k + 3] = w0.w;
-                x[8 * k + 4] = w1.x, x[8 * k + 5] = w1.y, x[8 * k + 6] = w1.z, x[8 * k + 7] = w1.w;
-            } else {
-                const h8_t w = *reinterpret_cast<const h8_t*>(src + 32 * k + 8 * g);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[8 * k + e] = (float)w[e];
-            }
-        }
-#pragma unroll
         for (int e = 0; e < 8 * NQ; ++e) {
-            x[e] = live ? x[e] : 0.f;
+            x[e] = live[ct] ? (float)rawq[ct][e / 8][e % 8] : 0.f;
             sum += x[e];
         }
         sum = add_rows(sum);

@@ -408,13 +408,8 @@ class PagedPool:
         return self.k.device
 
     def desc(self) -> VspecPagedKV:
-        d = VspecPagedKV()
-        d.dtype, d.num_blocks, d.block_tokens = self.dtype, self.num_blocks, self.block_tokens
-        d.num_kv_heads, d.head_dim = self.num_kv_heads, self.head_dim
-        d.k_data, d.v_data = self.k.data_ptr(), self.v.data_ptr()
-        d.k_scales, d.v_scales = _ptr(self.ks), _ptr(self.vs)
-        d.k_flags = _ptr(self.kf)
-        return d
+        return VspecPagedKV(self.dtype, self.num_blocks, self.block_tokens, self.num_kv_heads, self.head_dim,
+                            self.k.data_ptr(), self.v.data_ptr(), _ptr(self.ks), _ptr(self.vs), _ptr(self.kf))
 
 
 def kv_append(pool: PagedPool, block_tables, start_pos, k_new, v_new, stream=None):
@@ -663,21 +658,15 @@ def paged_tree_attention(pool: PagedPool, block_tables, start_pos, q, tree_mask=
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise VspecRocmError("paged_tree_attention: out must be as q")
-    d = VspecTreeAttnDesc()
-    d.kv = pool.desc()
-    d.batch, d.num_q_heads, d.num_nodes = B, Hq, N
-    d.block_tables, d.max_blocks_per_seq = bt.data_ptr(), bt.shape[1]
-    d.start_pos, d.max_start_pos = sp.data_ptr(), max_start_pos
-    d.tree_lens, d.tree_mask, d.block_used = _ptr(tl), _ptr(tree_mask), _ptr(bu)
-    d.q, d.out, d.io_dtype = q.data_ptr(), out.data_ptr(), _io_type("paged_tree_attention", q)
-    d.scale, d.numerics, d.clamp_alpha = scale, numerics, clamp_alpha
+    d = VspecTreeAttnDesc(pool.desc(), B, Hq, N, bt.data_ptr(), bt.shape[1], sp.data_ptr(), max_start_pos, _ptr(tl),
+                          _ptr(tree_mask), q.data_ptr(), out.data_ptr(), _io_type("paged_tree_attention", q), scale,
+                          numerics, clamp_alpha, None, 0, _stream(stream), _ptr(bu))
     if workspace is None:
         need = lib().vspec_rocm_paged_tree_attention_workspace_bytes(C.byref(d))
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     if workspace is not None:
         d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    d.stream = _stream(stream)
     _check(lib().vspec_rocm_paged_tree_attention(C.byref(d)), "paged_tree_attention")
     if stream is not None:
         _hold(stream, bt, sp, tl, bu, out, workspace)
@@ -726,32 +715,30 @@ def rope(positions, q=None, k=None, rope_dim=None, base=10000.0, layout=ROPE_HAL
     if q is None and k is None:
         raise VspecRocmError("rope: need q or k")
     first = q if q is not None else k
-    _on_device("rope", first.device, q=q, k=k, q_out=q_out, k_out=k_out)
-    pos = _i32(positions, first.device)
+    dev, dtype = first.device, first.dtype
+    _on_device("rope", dev, q=q, k=k, q_out=q_out, k_out=k_out)
+    pos = _i32(positions, dev)
+    if first.dim() != 3 or pos.numel() != first.shape[0]:
+        raise VspecRocmError("rope: rows must be [T][heads][D], and positions [T]")
     T, _, D = first.shape
-    d = VspecRopeDesc()
-    d.num_tokens, d.head_dim, d.rope_dim = T, D, D if rope_dim is None else rope_dim
-    d.dtype, d.layout, d.inverse = _io_type("rope", first), layout, int(inverse)
-    d.scaling, d.trained_len, d.base, d.factor = scaling, trained_len, base, factor
-    d.low, d.high, d.magnitude = low, high, magnitude
-    d.positions = pos.data_ptr()
+    d = VspecRopeDesc(T, D, D if rope_dim is None else rope_dim, _io_type("rope", first), layout, int(inverse), scaling,
+                      trained_len, base, factor, low, high, magnitude, pos.data_ptr())
+    d.stream = _stream(stream)
     outs = []
     for rows, x, out in ((d.q, q, q_out), (d.k, k, k_out)):
         if x is not None:
             if out is None:
-                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            for t in (x, out):
-                if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or t.dtype != first.dtype or t.stride(2) != 1:
-                    raise VspecRocmError("rope: rows must be [T][heads][D] of one type, the elements of a row adjacent")
-                if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
-                    raise VspecRocmError("rope: an expanded operand (stride 0) has no rows of its own")
-            if out.shape != x.shape or pos.numel() != T:
-                raise VspecRocmError("rope: positions, q, k and their outputs do not fit together")
-            rows.in_, rows.out, rows.num_heads = x.data_ptr(), out.data_ptr(), x.shape[1]
-            rows.in_token_stride, rows.in_head_stride = x.stride(0), x.stride(1)
-            rows.out_token_stride, rows.out_head_stride = out.stride(0), out.stride(1)
+                out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            shape = x.shape
+            if len(shape) != 3 or shape[0] != T or shape[2] != D or out.shape != shape or x.dtype != dtype or out.dtype != dtype:
+                raise VspecRocmError("rope: q, k and their outputs must be [T][heads][D] of one type")
+            a, b = x.stride(), out.stride()
+            if a[2] != 1 or b[2] != 1:
+                raise VspecRocmError("rope: the elements of a row must be adjacent")
+            if (T > 1 and (a[0] == 0 or b[0] == 0)) or (shape[1] > 1 and (a[1] == 0 or b[1] == 0)):
+                raise VspecRocmError("rope: an expanded operand (stride 0) has no rows of its own")
+            rows.__init__(x.data_ptr(), out.data_ptr(), shape[1], a[0], a[1], b[0], b[1])
         outs.append(out)
-    d.stream = _stream(stream)
     _check(lib().vspec_rocm_rope(C.byref(d)), "rope")
     if stream is not None:
         _hold(stream, pos, *outs)

@@ -5,6 +5,9 @@
 // 2^-33 turns at a million positions, and only its fraction goes on to the f32 sine and cosine
 // (in half turns, sincospif, so that no multiple of pi has to be taken away).  Every angle of a
 // token serves all its heads.
+//
+// What bounds it: reading and writing the rows, 16384 tokens of 40 heads, f16, D = 128, in 67 us,
+// 5.0 TB/s, the rate of a large copy; 256 tokens 6 us, launch and waits.
 #include <math.h>
 
 #include "host.h"
@@ -279,7 +282,7 @@ extern "C" int vspec_rocm_rope(const VspecRopeDesc* d) {
     const bool inter = d->layout == VSPEC_ROPE_INTERLEAVED, f32 = d->dtype == VSPEC_KV_F32;
     hipStream_t s = (hipStream_t)d->stream;
     // By chunks where rows, strides and the turned part are whole ones (16384 tokens of 40 heads: 215 us by
-    // elements, TIMED by chunks).  Tokens share a workgroup where that still leaves 4 to a CU.
+    // elements, 70 by chunks).  Tokens share a workgroup where that still leaves 4 to a CU.
     const uint32_t v = f32 ? 4 : 8, turned = inter ? d->rope_dim : d->rope_dim / 2;
     if (heads <= kChunkHeads && d->head_dim % v == 0 && turned % v == 0 && whole_chunks(p.q, v) && whole_chunks(p.k, v)) {
         RopeSplit w = {};

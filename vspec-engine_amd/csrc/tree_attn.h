@@ -249,8 +249,10 @@ void launch_tree_wide_int4_d128(const TreeParams& p, int32_t io, uint32_t ct, hi
 // 16-token tiles of a step
 constexpr int wide_step_tiles(bool f32_rows, int ct) { return f32_rows || ct > 1 ? 2 : 4; }
 constexpr int tree_step_tiles(int dtype) { return dtype == VSPEC_KV_F32 ? 1 : 2; }
-// Workgroups of tree_mfma.hip that a CU holds.  Two hide each other's waits, where 256 registers a
-// lane hold K, V, q and the output without spilling more than a few.
+// Workgroups of tree_mfma.hip that a CU holds.  Two hide each other's waits, and 256 registers a lane then hold K, V,
+// q and the output, but for up to 39 (int4, two tiles of f16 rows: 64 x 4097 tokens, 8 nodes 187 us with one workgroup,
+// 157 with two).  Two tiles of f32 rows would spill 68 and 90 (f16 and int4, 16 x 2049: 36 and 38 us with one, 50 and
+// 57 with two).
 constexpr int tree_cu_groups(int dtype, int d, bool f32_rows, int ct) {
     return ct == 1 || d == 64 || dtype == VSPEC_KV_F32 || !f32_rows ? 2 : 1;
 }

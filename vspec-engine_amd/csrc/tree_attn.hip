@@ -1,5 +1,5 @@
 // tree_attn.hip -- vspec_rocm_paged_tree_attention: its checks, its plan and its launches (the
-// kernels: tree_mfma.hip).
+// kernels: tree_mfma.hip, tree_wide.hip).
 #include <math.h>
 
 #include "host.h"
@@ -58,9 +58,14 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     TreePlan pl = {};
     const uint32_t cols = d->num_nodes * (d->num_q_heads / d->kv.num_kv_heads);
     const uint32_t tiles = (cols + 15) / 16;
+    // Up to two column tiles a wave keeps to itself (tree_mfma.hip); of more, waves share K and V through LDS
+    // (tree_wide.hip).  At 8 nodes of 4 heads, two tiles: 16 x 2049 tokens of an f16 pool 45 and 51 us, 64 x 4097 of
+    // an int4 pool 186 and 246; at 16 nodes, four tiles, the first kernel took 136 us where the second takes 49.
+    // f32 pools stay with the first: an exact clip of every key and f32 products, no operands
+    // in f16 to share.
     pl.wide = d->kv.dtype != VSPEC_KV_F32 && tiles > 2;
     if (pl.wide) {
-        pl.ct = tiles <= 4 ? 1 : 2;
+        pl.ct = tiles <= 4 ? 1 : 2;  // the least that holds them: a wave without columns reads and waits all the same
         pl.col_waves = tiles <= 8 ? 4 : 8;
     } else {
         pl.ct = tiles == 1 ? 1 : 2;
@@ -73,6 +78,7 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     const bool f32_rows = d->io_dtype == VSPEC_KV_F32;
     // a unit: a step, or one of each of the waves that share a row's steps
     const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype) * (4 / pl.col_waves));
+    // (of 1 and 2 without sharing: one sequence of 700 tokens 13.3 and 14.6 us, 16 of 500 17.6 and 15.9)
     pl.min_units = pl.wide ? 4 : 1;
     const uint64_t batch = d->batch, units = (bound + per - 1) / per;
     const uint64_t items = (uint64_t)d->kv.num_kv_heads * pl.col_groups;

@@ -217,9 +217,10 @@ typedef struct VspecTreeAttnDesc {
                                         only the rows that see it, whatever their bits */
     const void* q;                   /* device [batch][N][Hq][D] in io_dtype, 16-byte aligned */
     void* out;                       /* device, as q */
-    int32_t io_dtype;                /* VSPEC_KV_F32 or VSPEC_KV_F16.  f16 rows are multiplied
-                                        with softmax weights rounded to f16 (and int4 values
-                                        rounded to f16); f32 rows keep about 22 bits */
+    int32_t io_dtype;                /* VSPEC_KV_F32 or VSPEC_KV_F16.  f32 rows keep about 22
+                                        bits throughout; f16 rows may be multiplied with
+                                        softmax weights and int4 values rounded to f16, each
+                                        an error like that of rounding the output */
     float scale;                     /* <= 0: 1/sqrtf(D) */
     int32_t numerics;                /* VSPEC_NUMERICS_PLAIN or VSPEC_NUMERICS_3BIT */
     float clamp_alpha;               /* <= 0: 4.5 */
@@ -241,7 +242,8 @@ int vspec_rocm_paged_tree_attention(const VspecTreeAttnDesc* desc);
  * the pools share dtype, geometry and block tables).  Any order of nodes is right, the same
  * node twice included.  new_lens (device int32 [batch], or NULL) gets start_pos[b] plus the
  * accepted nodes.  A slot outside the table or behind an invalid entry is neither read nor
- * written.  The blocks written belong to their sequence alone.  max_path and num_nodes are at
+ * written.  The blocks written belong to their sequence alone: a group of 4 slots of V that a
+ * destination lies in is written whole, the other slots as they were.  max_path and num_nodes are at
  * most 64. */
 int vspec_rocm_kv_accept(const VspecPagedKV* kvs, uint32_t num_kvs, uint32_t batch,
                          const int32_t* block_tables, uint32_t max_blocks_per_seq,

@@ -10,8 +10,14 @@
 // so neither scores nor weights pass through LDS.  f16 and int4 pools use 16x16x32 f16 MFMAs
 // (the 8 tokens of a lane in a step are tokens 4g..4g+3 of two tiles), f32 pools 16x16x4 f32.
 //
-// Precision.  f32 rows (IO = float) keep 22 bits of q and p, each split in two f16 (hi + lo), and
-// of int4 values; f16 rows take q, p and int4 values rounded to f16 once.  Sums are f32.  p is
+// Precision.  f32 rows (IO = float) keep 22 bits of q, p and an int4 pool's keys and values, each
+// split in two f16 (hi + lo).  f16 rows are exact in f16 and come out rounded to it, 2.1e-4 of the
+// output's norm; one more rounding of each weight (f16 pools) makes that 2.5e-4 to 2.9e-4.  Of int4
+// pools, rounding weights, keys (a code times a scale has 15 bits) and values once each would make
+// it 3.7e-4, so there keys keep their low parts, and weights too: 2.7e-4, for 10 % of the time of
+// one column tile and 30 % of 64 nodes' (64 x 4097 tokens: 118 -> 130 and 550 -> 720 us).  Two
+// tiles a wave leave out the weights' low parts for want of registers (160 -> 174 us, with them
+// 194): 3.0e-4.  Sums are f32.  p is
 // scaled by 2^kHeadroom against the reference point of the softmax, which follows the maximum
 // only when that has grown by 2^8, so p <= 2^11 fits f16 and weights down to 2^-27 of the
 // largest count.
@@ -63,8 +69,10 @@ struct Tile<VSPEC_KV_F32, D> {
 template <int DT, int D, typename IO, int CT>
 __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) void tree_attention(TreeParams p) {
     constexpr bool F32 = DT == VSPEC_KV_F32;
-    constexpr bool SPLIT = sizeof(IO) == 4 && !F32;      // q and p in two f16 parts
-    constexpr bool VLO = SPLIT && DT == VSPEC_KV_INT4;   // K and V in two f16 parts
+    constexpr bool SPLIT = sizeof(IO) == 4 && !F32;      // q in two f16 parts
+    constexpr bool KLO = DT == VSPEC_KV_INT4;            // K in two f16 parts
+    constexpr bool PLO = SPLIT || (DT == VSPEC_KV_INT4 && CT == 1);  // p in two f16 parts
+    constexpr bool VLO = SPLIT && DT == VSPEC_KV_INT4;   // V in two f16 parts
     constexpr int NT = tree_step_tiles(DT);
     constexpr int NQ = D / 32;   // f16 score MFMAs of a tile
     constexpr int NDT = D / 16;  // d-tiles of the output
@@ -310,14 +318,14 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
         const bool masked = step >= tp.prefix_steps || s.valid[0] < kTile || s.valid[NT - 1] < kTile;
         const int tile0 = first_tile(step);
         // ---- K operands, each key held to its own limit ----
-        h8_t kh[F32 ? 1 : NT][NQ], kl[SPLIT ? NT : 1][NQ];
+        h8_t kh[F32 ? 1 : NT][NQ], kl[SPLIT || KLO ? NT : 1][NQ];
         bool low[NT];    // kl holds something
         float kunit[NT]; // scores come out divided by this
         bool nans[NT];   // a key may be NaN
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
             T& t = tile[a];
-            low[a] = VLO;
+            low[a] = KLO;
             kunit[a] = 1.f;
             nans[a] = F32;
             if constexpr (F32) {
@@ -372,7 +380,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                             const h2_t y = q4[c] * s2v;
                             kh[a][i][2 * c] = y[0];
                             kh[a][i][2 * c + 1] = y[1];
-                            if constexpr (VLO) {
+                            if constexpr (KLO) {
                                 const h2_t z = __builtin_elementwise_fma(q4[c], s2v, -y);  // exact
                                 kl[a][i][2 * c] = z[0];
                                 kl[a][i][2 * c + 1] = z[1];
@@ -395,7 +403,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                     // the flagged keys (any lane of token n flags it), exactly: two-pass deviation, and the clipped row
                     // in two f16 parts.  Elements inside the limit stay exact, the limit keeps 22 bits or 2^-25.
                     nans[a] = true;
-                    low[a] = SPLIT;
+                    low[a] = SPLIT || KLO;
                     const bool mine = ((any | (any >> 16) | (any >> 32) | (any >> 48)) >> n) & 1u;
                     float x[8 * NQ], sum = 0.f, var = 0.f;
 #pragma unroll
@@ -426,9 +434,9 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                             y = (y != y ? y : __builtin_amdgcn_fmed3f(y, -th, th)) * down;
                             const _Float16 y16 = (_Float16)y;
                             kh[a][i][e] = mine ? y16 : kh[a][i][e];
-                            if constexpr (SPLIT) {
+                            if constexpr (SPLIT || KLO) {
                                 const _Float16 z16 = (_Float16)(y - (float)y16);
-                                kl[a][i][e] = mine ? z16 : VLO ? kl[a][i][e] : (_Float16)0.f;
+                                kl[a][i][e] = mine ? z16 : KLO ? kl[a][i][e] : (_Float16)0.f;
                             }
                         }
                     }
@@ -451,7 +459,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
 #pragma unroll
                         for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[a][i], ql[ct][i], c, 0, 0, 0);
                     }
-                    if constexpr (VLO) {
+                    if constexpr (KLO) {
 #pragma unroll
                         for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[a][i], qh[ct][i], c, 0, 0, 0);
                     }
@@ -461,7 +469,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                 sc[ct][a] = c;
             }
         }
-        if constexpr (SPLIT && !VLO) {
+        if constexpr (SPLIT && !KLO) {
 #pragma unroll
             for (int a = 0; a < NT; ++a) {
                 if (!low[a]) continue;
@@ -533,7 +541,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                 for (int j = 0; j < NDT; ++j) acc[ct][j] *= f;
             }
         }
-        h8_t ph[F32 ? 1 : CT], pl[SPLIT ? CT : 1];
+        h8_t ph[F32 ? 1 : CT], pl[PLO ? CT : 1];
         float pf[F32 ? CT : 1][4];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -546,7 +554,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                 } else {
                     const _Float16 w16 = (_Float16)w;
                     ph[ct][e] = w16;
-                    if constexpr (SPLIT) pl[ct][e] = (_Float16)(w - (float)w16);
+                    if constexpr (PLO) pl[ct][e] = (_Float16)(w - (float)w16);
                 }
             }
         }
@@ -640,7 +648,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
                     acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct], acc[ct][j], 0, 0, 0);
-                    if constexpr (SPLIT) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct], acc[ct][j], 0, 0, 0);
+                    if constexpr (PLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct], acc[ct][j], 0, 0, 0);
                     if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph[ct], acc[ct][j], 0, 0, 0);
                 }
             }
@@ -676,7 +684,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                         for (int j = 0; j < NDT; ++j) {
                             const h8_t v = join(vh[0][j], vh[NT - 1][j]);
                             acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph16, acc[ct][j], 0, 0, 0);
-                            if constexpr (SPLIT) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct] * up8, acc[ct][j], 0, 0, 0);
+                            if constexpr (PLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct] * up8, acc[ct][j], 0, 0, 0);
                             if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph16, acc[ct][j], 0, 0, 0);
                         }
                     }

@@ -9,7 +9,7 @@
 //         that loaded a key's row screens it for the clip to its own standard deviation, rewrites a
 //         clipped row in place and leaves its low part beside it.
 //   int4  codes and scales stream into a ring of each wave; it turns its share of a step into f16
-//         rows (and their low parts, for f32 queries) in LDS, clipped on the way.
+//         rows, keys with their low parts (values for f32 queries), in LDS, clipped on the way.
 // A wave's column then costs per 32 tokens its matrix instructions, 8 weights a lane and 16 reads
 // of 16 bytes from LDS.  With CT = 2 and 8 waves the LDS reads (128 KB a step, 1024 cycles) are as
 // long as the f16 matrix work of 256 columns; with one tile a wave they would be twice that.
@@ -45,8 +45,10 @@ constexpr bool SPLIT_IO = sizeof(IO) == 4;
 template <int DT, int D, typename IO, int CT, int W>
 __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree_wide(TreeParams p) {
     constexpr bool F16 = DT == VSPEC_KV_F16;
-    constexpr bool SPLIT = SPLIT_IO<IO>;      // q and p in two f16 parts
-    constexpr bool VLO = SPLIT && !F16;       // K and V in two f16 parts
+    constexpr bool SPLIT = SPLIT_IO<IO>;      // q in two f16 parts
+    constexpr bool KLO = !F16;                // K in two f16 parts
+    constexpr bool PLO = SPLIT || !F16;       // p in two f16 parts
+    constexpr bool VLO = SPLIT && !F16;       // V in two f16 parts
     constexpr int NQ = D / 32, NDT = D / 16;
     constexpr int KT = wide_step_tiles(SPLIT, CT);  // 16-token tiles of a step
     constexpr int CPT = D / 8;                // 8-element chunks of a row
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
     constexpr int RAW = 3;                    // steps of codes in the ring
     constexpr int kRawB = F16 ? 16 : 512 * SETS + 512;  // of a wave and step: K, V, K scales, V scales
     __shared__ __align__(16) uint8_t stage[DEPTH * kStageB];
-    __shared__ __align__(16) uint8_t low[SPLIT ? (F16 ? 2 * KT * kTileB : kStageB) : 16];  // low parts: f16 [mark][K], int4 as a stage
+    __shared__ __align__(16) uint8_t low[F16 ? (SPLIT ? 2 * KT * kTileB : 16) : (VLO ? kStageB : KT * kTileB)];  // low parts: f16 [mark][K], int4 as a stage
     __shared__ __align__(16) uint8_t raw[F16 ? 16 : RAW * OWNERS * kRawB];
     // a bit for each row of a step, whole bytes of each wave's: clipped or not finite; K (int4) and V (int4) hold a 16th of the
     // value; V held something that is not finite
@@ -296,10 +298,8 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                 for (int e = 0; e < 4; ++e) {
                     const h2_t y = q4[e] * s2v;
                     yh[2 * e] = y[0], yh[2 * e + 1] = y[1];
-                    if constexpr (VLO) {
-                        const h2_t z = __builtin_elementwise_fma(q4[e], s2v, -y);  // exact
-                        yl[2 * e] = z[0], yl[2 * e + 1] = z[1];
-                    }
+                    const h2_t z = __builtin_elementwise_fma(q4[e], s2v, -y);  // exact
+                    yl[2 * e] = z[0], yl[2 * e + 1] = z[1];
                 }
                 const uint64_t any = __builtin_amdgcn_ballot_w64(flag && row < valid);
                 if (any != 0) {
@@ -324,13 +324,13 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                         const float y = (x[e] != x[e] ? x[e] : __builtin_amdgcn_fmed3f(x[e], -th, th)) * down;
                         const _Float16 y16 = (_Float16)y, z16 = (_Float16)(y - (float)y16);
                         yh[e] = mine_too ? y16 : yh[e];
-                        if constexpr (VLO) yl[e] = mine_too ? z16 : yl[e];
+                        yl[e] = mine_too ? z16 : yl[e];
                     }
                 }
                 const int m = row / TI, t = row % TI;
                 const int at = my_tile * kTileB + m * 1024 + (CPT * t + chunk_of<D>(m, CPT * t + c)) * 16;
                 *reinterpret_cast<h8_t*>(stage + at) = yh;
-                if constexpr (VLO) *reinterpret_cast<h8_t*>(low + at) = yl;
+                *reinterpret_cast<h8_t*>(low + at) = yl;
             }
 #pragma unroll
             for (int k = 0; k < SETS; ++k) {
@@ -493,11 +493,11 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
         const bool masked = step >= tp.prefix_steps || tokens != (KT == 4 ? 0x84210 : 0x210);
 #pragma unroll
         for (int a = 0; a < KT; ++a) {
-            h8_t kh[NQ], kl[VLO ? NQ : 1];
+            h8_t kh[NQ], kl[KLO ? NQ : 1];
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 kh[i] = *reinterpret_cast<const h8_t*>(st + a * kTileB + (kread ^ (64 * i)));
-                if constexpr (VLO) kl[i] = *reinterpret_cast<const h8_t*>(low + a * kTileB + (kread ^ (64 * i)));
+                if constexpr (KLO) kl[i] = *reinterpret_cast<const h8_t*>(low + a * kTileB + (kread ^ (64 * i)));
             }
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[i], ql[ct][i], c, 0, 0, 0);
                 }
-                if constexpr (VLO) {
+                if constexpr (KLO) {
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[i], qh[ct][i], c, 0, 0, 0);
                 }
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                 for (int j = 0; j < NDT; ++j) acc[ct][j] *= f;
             }
         }
-        h8_t ph[CT][KT / 2], pl[SPLIT ? CT : 1][KT / 2];
+        h8_t ph[CT][KT / 2], pl[PLO ? CT : 1][KT / 2];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
@@ -595,12 +595,12 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                     const float w = __builtin_amdgcn_exp2f(fmaf(sc[ct][2 * u + e / 4][e % 4], fac[ct], -mf[ct]));
                     const _Float16 w16 = (_Float16)w;
                     ph[ct][u][e] = w16;
-                    if constexpr (SPLIT) pl[ct][u][e] = (_Float16)(w - (float)w16);
+                    if constexpr (PLO) pl[ct][u][e] = (_Float16)(w - (float)w16);
                 }
                 const _Float16 o = (_Float16)1.f;
                 const h8_t ones = {o, o, o, o, o, o, o, o};
                 total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[ct][u], total[ct], 0, 0, 0);
-                if constexpr (SPLIT) total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[ct][u], total[ct], 0, 0, 0);
+                if constexpr (PLO) total[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[ct][u], total[ct], 0, 0, 0);
             }
         }
         if constexpr (!F16) {
@@ -613,7 +613,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                         for (int e = 0; e < 8; ++e) {
                             const _Float16 up = (tile_marks(vb, 2 * u + e / 4) >> (4 * g + e % 4)) & 1u ? (_Float16)16.f : (_Float16)1.f;
                             ph[ct][u][e] *= up;
-                            if constexpr (SPLIT) pl[ct][u][e] *= up;
+                            if constexpr (PLO) pl[ct][u][e] *= up;
                         }
                     }
                 }
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree
                     for (int ct = 0; ct < CT; ++ct) {
                         f4_t& c = acc[ct][2 * i + o];
                         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, ph[ct][u], c, 0, 0, 0);
-                        if constexpr (SPLIT) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, pl[ct][u], c, 0, 0, 0);
+                        if constexpr (PLO) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, pl[ct][u], c, 0, 0, 0);
                         if constexpr (VLO) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, ph[ct][u], c, 0, 0, 0);
                     }
                 }

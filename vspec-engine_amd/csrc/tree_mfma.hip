@@ -14,10 +14,9 @@
 // split in two f16 (hi + lo).  f16 rows are exact in f16 and come out rounded to it, 2.1e-4 of the
 // output's norm; one more rounding of each weight (f16 pools) makes that 2.5e-4 to 2.9e-4.  Of int4
 // pools, rounding weights, keys (a code times a scale has 15 bits) and values once each would make
-// it 3.7e-4, so there keys keep their low parts, and weights too: 2.7e-4, for 10 % of the time of
-// one column tile and 30 % of 64 nodes' (64 x 4097 tokens: 118 -> 130 and 550 -> 720 us).  Two
-// tiles a wave leave out the weights' low parts for want of registers (160 -> 174 us, with them
-// 194): 3.0e-4.  Sums are f32.  p is
+// it 3.7e-4, so there keys and weights keep their low parts, 2.7e-4, for 10 % of the time of few
+// nodes and 30 % of 64 nodes' (64 x 4097 tokens: 4 nodes 118 -> 134, 8 160 -> 177, 64 550 -> 715
+// us).  Sums are f32.  p is
 // scaled by 2^kHeadroom against the reference point of the softmax, which follows the maximum
 // only when that has grown by 2^8, so p <= 2^11 fits f16 and weights down to 2^-27 of the
 // largest count.
@@ -39,6 +38,8 @@
 // 190 us, 5.7 TB/s.  int4 pools: the vector instructions that turn codes into f16 and screen the
 // keys, 2.6 TB/s there.  Short sequences: the chain of launch, lengths, table, tile and join, 13 us
 // for one sequence of 100 to 3000 tokens, of which 3 are the next launch's.
+#include <type_traits>
+
 #include "tree_common.h"
 
 namespace vkv {
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
     constexpr bool F32 = DT == VSPEC_KV_F32;
     constexpr bool SPLIT = sizeof(IO) == 4 && !F32;      // q in two f16 parts
     constexpr bool KLO = DT == VSPEC_KV_INT4;            // K in two f16 parts
-    constexpr bool PLO = SPLIT || (DT == VSPEC_KV_INT4 && CT == 1);  // p in two f16 parts
+    constexpr bool PLO = SPLIT || DT == VSPEC_KV_INT4;   // p in two f16 parts
     constexpr bool VLO = SPLIT && DT == VSPEC_KV_INT4;   // V in two f16 parts
     constexpr int NT = tree_step_tiles(DT);
     constexpr int NQ = D / 32;   // f16 score MFMAs of a tile
@@ -589,36 +590,68 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                 }
             }
         } else {
-            h4_t vh[NT][NDT], vl[VLO ? NT : 1][NDT];
-            bool big = false;
-            if constexpr (DT == VSPEC_KV_INT4) {
-                bool mine_big = false;
+            // acc += V^T p of d-tile j
+            auto add_values = [&](const int j, const h8_t v, const h8_t vl, const h8_t (&ph)[CT], const h8_t (&pl)[PLO ? CT : 1]) {
 #pragma unroll
-                for (int a = 0; a < NT; ++a) {
-                    bool mine = false;
+                for (int ct = 0; ct < CT; ++ct) {
+                    acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct], acc[ct][j], 0, 0, 0);
+                    if constexpr (PLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct], acc[ct][j], 0, 0, 0);
+                    if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[ct], acc[ct][j], 0, 0, 0);
+                }
+            };
+            if constexpr (DT == VSPEC_KV_INT4) {
+                // word c of the lane's chunks at a time: values of d-tiles 2c and 2c + 1.  In the products of scales of 2^12
+                // and more (LARGE: of no others) a code may pass f16's range: they are left for a pass of their own, over 2^4,
+                // with p 2^4 (p <= 2^11).
+                auto values = [&](auto large_tag, const h8_t (&ph)[CT], const h8_t (&pl)[PLO ? CT : 1]) -> bool {
+                    constexpr bool LARGE = decltype(large_tag)::value;
+                    bool mine_big = false, mine = false;
 #pragma unroll
                     for (int c = 0; c < NQ; ++c) {
-                        h2_t sp2[2];
+                        h4_t vh[NT][2], vl[NT][2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            // in the products of scales of 2^12 and more a code may pass f16's range: they are left
-                            // for a product of their own
-                            uint32_t w = int4_scale_pair<NQ>(tile[a], c, e);
-                            if (s.valid[a] < kTile) {
-                                w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
+                        for (int a = 0; a < NT; ++a) {
+                            h2_t sp2[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                uint32_t w = int4_scale_pair<NQ>(tile[a], c, e);
+                                if (s.valid[a] < kTile) {
+                                    w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
+                                }
+                                const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
+                                if constexpr (LARGE) {
+                                    const bool l_in = lo16 >= kBigScale && (!tree[a] || lo16 < 0x7C00u), h_in = hi16 >= kBigScale && (!tree[a] || hi16 < 0x7C00u);
+                                    w &= (l_in ? 0xffffu : 0u) | (h_in ? 0xffff0000u : 0u);
+                                    const h2_t down = {(_Float16)0.0625f, (_Float16)0.0625f};
+                                    sp2[e] = __builtin_bit_cast(h2_t, w) * down;
+                                } else {
+                                    mine_big = mine_big || max(lo16, hi16) >= kBigScale;
+                                    mine = mine || (tree[a] && max(lo16, hi16) >= 0x7C00u);
+                                    w &= (lo16 < kBigScale ? 0xffffu : 0u) | (hi16 < kBigScale ? 0xffff0000u : 0u);
+                                    sp2[e] = __builtin_bit_cast(h2_t, w);
+                                }
                             }
-                            const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
-                            mine_big = mine_big || max(lo16, hi16) >= kBigScale;
-                            mine = mine || (tree[a] && max(lo16, hi16) >= 0x7C00u);
-                            w &= (lo16 < kBigScale ? 0xffffu : 0u) | (hi16 < kBigScale ? 0xffff0000u : 0u);
-                            sp2[e] = __builtin_bit_cast(h2_t, w);
+                            int4_values<VLO>(tile[a].v[c], sp2, vh[a][0], vh[a][1], vl[a][0], vl[a][1]);
                         }
-                        int4_values<VLO>(tile[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
+#pragma unroll
+                        for (int o = 0; o < 2; ++o) add_values(2 * c + o, join(vh[0][o], vh[NT - 1][o]), join(vl[0][o], vl[NT - 1][o]), ph, pl);
                     }
                     wild = wild || __builtin_amdgcn_ballot_w64(mine) != 0;
+                    return __builtin_amdgcn_ballot_w64(mine_big) != 0;
+                };
+                if (values(std::false_type(), ph, pl)) {
+                    const _Float16 up = (_Float16)16.f;
+                    const h8_t up8 = {up, up, up, up, up, up, up, up};
+                    h8_t ph16[CT], pl16[CT];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        ph16[ct] = ph[ct] * up8;
+                        pl16[ct] = pl[ct] * up8;
+                    }
+                    values(std::true_type(), ph16, pl16);
                 }
-                big = __builtin_amdgcn_ballot_w64(mine_big) != 0;
             } else {
+                h4_t vh[NT][NDT];
 #pragma unroll
                 for (int a = 0; a < NT; ++a) {
 #pragma unroll
@@ -641,53 +674,10 @@ __global__ __launch_bounds__(256, tree_cu_groups(DT, D, sizeof(IO) == 4, CT)) vo
                         wild = wild || __builtin_amdgcn_ballot_w64(mine) != 0;
                     }
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < NDT; ++j) {
-                const h8_t v = join(vh[0][j], vh[NT - 1][j]);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[ct], acc[ct][j], 0, 0, 0);
-                    if constexpr (PLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct], acc[ct][j], 0, 0, 0);
-                    if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph[ct], acc[ct][j], 0, 0, 0);
-                }
-            }
-            if constexpr (DT == VSPEC_KV_INT4) {
-                if (big) {
-                    // the large values over 2^4 times p 2^4 (p <= 2^11)
-                    const h2_t down = {(_Float16)0.0625f, (_Float16)0.0625f};
-#pragma unroll
-                    for (int a = 0; a < NT; ++a) {
-#pragma unroll
-                        for (int c = 0; c < NQ; ++c) {
-                            h2_t sp2[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                uint32_t w = int4_scale_pair<NQ>(tile[a], c, e);
-                                if (s.valid[a] < kTile) {
-                                    w &= (4 * g + 2 * e < s.valid[a] ? 0xffffu : 0u) | (4 * g + 2 * e + 1 < s.valid[a] ? 0xffff0000u : 0u);
-                                }
-                                const uint32_t lo16 = w & 0x7fffu, hi16 = (w >> 16) & 0x7fffu;
-                                const bool l_in = lo16 >= kBigScale && (!tree[a] || lo16 < 0x7C00u), h_in = hi16 >= kBigScale && (!tree[a] || hi16 < 0x7C00u);
-                                w &= (l_in ? 0xffffu : 0u) | (h_in ? 0xffff0000u : 0u);
-                                sp2[e] = __builtin_bit_cast(h2_t, w) * down;
-                            }
-                            int4_values<VLO>(tile[a].v[c], sp2, vh[a][2 * c], vh[a][2 * c + 1], vl[VLO ? a : 0][2 * c], vl[VLO ? a : 0][2 * c + 1]);
-                        }
-                    }
-                    const _Float16 up = (_Float16)16.f;
-                    const h8_t up8 = {up, up, up, up, up, up, up, up};
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        const h8_t ph16 = ph[ct] * up8;
-#pragma unroll
-                        for (int j = 0; j < NDT; ++j) {
-                            const h8_t v = join(vh[0][j], vh[NT - 1][j]);
-                            acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph16, acc[ct][j], 0, 0, 0);
-                            if constexpr (PLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[ct] * up8, acc[ct][j], 0, 0, 0);
-                            if constexpr (VLO) acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(join(vl[0][j], vl[NT - 1][j]), ph16, acc[ct][j], 0, 0, 0);
-                        }
-                    }
+                for (int j = 0; j < NDT; ++j) {
+                    const h8_t v = join(vh[0][j], vh[NT - 1][j]);
+                    add_values(j, v, v, ph, pl);
                 }
             }
         }

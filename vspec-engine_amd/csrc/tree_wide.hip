@@ -43,7 +43,7 @@ template <typename IO>
 constexpr bool SPLIT_IO = sizeof(IO) == 4;
 
 template <int DT, int D, typename IO, int CT, int W>
-__global__ __launch_bounds__(W * 64, CT == 1 && !SPLIT_IO<IO> ? 3 : 2) void tree_wide(TreeParams p) {
+__global__ __launch_bounds__(W * 64, 2) void tree_wide(TreeParams p) {
     constexpr bool F16 = DT == VSPEC_KV_F16;
     constexpr bool SPLIT = SPLIT_IO<IO>;      // q in two f16 parts
     constexpr bool KLO = !F16;                // K in two f16 parts

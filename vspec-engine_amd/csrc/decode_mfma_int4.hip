@@ -34,7 +34,7 @@
 // The std clamp is screened per key from v_dot8 sums of the codes (sum c, sum c^2)
 // and the bound |x| <= 8 * scale; keys it may affect get exact fp32 scores.
 #include "append_row.h"
-#include "kv_common.h"
+#include "lds_load.h"
 
 namespace vkv {
 namespace {

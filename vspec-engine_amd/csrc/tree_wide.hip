@@ -16,6 +16,7 @@
 //
 // One barrier a step orders the ring (f16): a wave issues the loads of step s + DEPTH - 1 into the
 // slot of step s - 1, which every wave left before the last barrier.
+#include "lds_load.h"
 #include "tree_common.h"
 
 namespace vkv {

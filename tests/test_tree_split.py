@@ -205,3 +205,23 @@ def test_rope_sizes(vr, io, layout, T, Hq, Hk, D, R):
             continue
         _near(y, _rotated(x, pos, R, layout, speeds, m, False))
         assert torch.equal(y[..., R:], x[..., R:])
+
+
+@DTYPES
+def test_nothing_to_do(vr, dtype):
+    """No tokens, no sequences, a path without entries."""
+    import torch
+
+    for t in (torch.float32, torch.float16):
+        q, k = (torch.empty((0, h, 64), dtype=t, device="cuda") for h in (4, 1))
+        a, b = vr.rope(_int([]), q, k)
+        assert a.shape == q.shape and b.shape == k.shape
+    c = Cache(vr, dtype, [20], 4, 1, 64, 16, seed=97)
+    before = _raw(vr, c.pool)
+    none = torch.empty((0, c.tables.shape[1]), dtype=torch.int32, device="cuda")
+    out = vr.paged_tree_attention(c.pool, none, _int([]), torch.empty((0, 4, 4, 64), device="cuda"))
+    assert out.shape == (0, 4, 4, 64)
+    assert vr.kv_accept([c.pool], none, _int([]), torch.empty((0, 4), dtype=torch.int32, device="cuda"), 4).numel() == 0
+    assert vr.kv_accept([c.pool], c.tables, c.start, torch.empty((1, 0), dtype=torch.int32, device="cuda"), 4).tolist() == [20]
+    for a, b in zip(before, _raw(vr, c.pool)):
+        assert torch.equal(a, b)

@@ -207,3 +207,8 @@ def test_binding_refusals(vr):
             vr.PagedPool.over(*args)
     with pytest.raises(ValueError):
         vr.PagedPool.over(7, 16, 1, 64, k, k)
+
+
+def test_rope_no_tokens_no_addresses(vr):
+    """Empty tensors have no address: nothing to do, not an error."""
+    assert vr.lib().vspec_rocm_rope(C.byref(_rope(vr, num_tokens=0, positions=None, q_in_=None, q_out=None))) == 1

@@ -263,13 +263,14 @@ extern "C" int vspec_rocm_rope(const VspecRopeDesc* d) {
     }
     RopeParams p = {};
     if (!rope_turns(d, p.turns, &p.magnitude)) return 0;
+    if (d->num_tokens == 0) return 1;  // (empty tensors have no address)
     if (!rope_operand(&d->q, d, "q", &p.q) || !rope_operand(&d->k, d, "k", &p.k)) return 0;
     const uint64_t heads = (uint64_t)p.q.heads + p.k.heads;
     if (heads > 65536u || d->num_tokens > 0x7fffffffu) {
         host_error("rope: at most 65536 heads and 2^31 - 1 tokens");
         return 0;
     }
-    if (d->num_tokens == 0 || heads == 0) return 1;
+    if (heads == 0) return 1;
     if (!d->positions) {
         host_error("rope: null positions");
         return 0;

@@ -64,17 +64,22 @@ TreePlan plan_tree(const VspecTreeAttnDesc* d) {
     // f32 pools stay with the first: an exact clip of every key and f32 products, no operands
     // in f16 to share.
     pl.wide = d->kv.dtype != VSPEC_KV_F32 && tiles > 2;
+    const uint64_t cap = (uint64_t)d->max_blocks_per_seq * d->kv.block_tokens;
+    uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
+    if (bound > cap) bound = cap;
     if (pl.wide) {
         pl.ct = tiles <= 4 ? 1 : 2;  // the least that holds them: a wave without columns reads and waits all the same
         pl.col_waves = tiles <= 8 ? 4 : 8;
     } else {
-        pl.ct = tiles == 1 ? 1 : 2;
-        pl.col_waves = tiles <= 2 ? 1 : tiles <= 4 ? 2 : 4;
+        // Two tiles to a wave read K and V once, which counts where they are long (64 x 4097 tokens, 8 nodes: f16 208 us,
+        // int4 177; by two waves side by side 245 and 226); two waves have less to do in a row each, which counts where
+        // a CU gets few tokens (one sequence of 700, 5 nodes: 11 us and 10, by one wave 13 and 12.6; 16 x 500, 250 tokens
+        // a CU: 21.6 and 20.7).
+        const bool beside = tiles == 2 && bound * d->batch * d->kv.num_kv_heads <= 128ull * host_num_cus();
+        pl.ct = tiles == 1 || beside ? 1 : 2;
+        pl.col_waves = (tiles + pl.ct - 1) / pl.ct > 2 ? 4 : (tiles + pl.ct - 1) / pl.ct;
     }
     pl.col_groups = (tiles + pl.ct * pl.col_waves - 1) / (pl.ct * pl.col_waves);
-    const uint64_t cap = (uint64_t)d->max_blocks_per_seq * d->kv.block_tokens;
-    uint64_t bound = (d->max_start_pos ? d->max_start_pos : cap) + d->num_nodes;
-    if (bound > cap) bound = cap;
     const bool f32_rows = d->io_dtype == VSPEC_KV_F32;
     // a unit: a step, or one of each of the waves that share a row's steps
     const uint32_t per = 16 * (pl.wide ? wide_step_tiles(f32_rows, pl.ct) : tree_step_tiles(d->kv.dtype) * (4 / pl.col_waves));

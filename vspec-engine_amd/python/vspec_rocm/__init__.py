@@ -306,8 +306,8 @@ def _stream(stream=None):
     a raw handle."""
     import torch
 
-    if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+    if stream is None:  # (the handle alone: a Stream object takes 3 us to make)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream
     return int(stream)

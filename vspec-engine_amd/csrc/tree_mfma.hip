@@ -32,12 +32,12 @@
 // Waits.  K's registers take the next step's rows as soon as the scores are there, V's at the end
 // of the step, and a second workgroup on the CU fills what is left (tree_cu_groups).  With a whole
 // step ahead in registers and one workgroup, 64 x 4097 tokens of an int4 pool, 4 nodes of 4 query
-// heads, took 154 us; this takes 115.
+// heads, took 154 us; this took 115 (134 now that their weights and keys have low parts).
 //
 // What bounds it (GQA 32 / 8, D = 128).  f16 pools: reading them, 64 x 4097 tokens and 4 nodes in
 // 190 us, 5.7 TB/s.  int4 pools: the vector instructions that turn codes into f16 and screen the
-// keys, 2.6 TB/s there.  Short sequences: the chain of launch, lengths, table, tile and join, 13 us
-// for one sequence of 100 to 3000 tokens, of which 3 are the next launch's.
+// keys, 2.3 TB/s there (134 us).  Short sequences: the chain of lengths, table, tile and join, and the
+// fetch of the code itself, 11 to 13 us for one sequence of 100 to 3000 tokens.
 #include <type_traits>
 
 #include "tree_common.h"
